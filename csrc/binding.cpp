@@ -381,6 +381,7 @@ torch::Tensor read_status(torch::Tensor workspace, int64_t cp_rank, int64_t cp_s
 // defined in binding_ops.cpp: attention / o_proj / fused ops
 void register_compute_ops(torch::Library& m);
 void bind_compute(pybind11::module_& m);
+void register_paged_ops(torch::Library& m);
 
 TORCH_LIBRARY(helix_a2a_b200, m) {
   m.def("get_helix_workspace_size_per_rank(int cp_size) -> int", &get_helix_workspace_size_per_rank);
@@ -402,6 +403,7 @@ TORCH_LIBRARY(helix_a2a_b200, m) {
   m.def("lse_combine(Tensor outputs, Tensor lses, int rank_dim, bool return_lse, bool base2) -> (Tensor, Tensor)",
         &lse_combine);
   register_compute_ops(m);
+  register_paged_ops(m);
 }
 
 // ---- pybind module: allocator + host utilities ---------------------------------------------------

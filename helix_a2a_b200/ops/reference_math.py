@@ -224,3 +224,60 @@ def mla_partial_attention(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv: torch.T
     if base2:
         lse = lse * LOG2E
     return o, lse
+
+
+# ----------------------------------------------------------------------------------------
+# new tokens of a step: pages, slots, masks, cache writes
+# ----------------------------------------------------------------------------------------
+
+def local_tokens(n: int, cp_size: int, cp_rank: int, interleave: int) -> int:
+    """How many of a sequence's first ``n`` tokens rank ``cp_rank`` holds (token p is on rank ``p // interleave % cp_size``)."""
+    cycle = interleave * cp_size
+    return n // cycle * interleave + min(max(n % cycle - cp_rank * interleave, 0), interleave)
+
+
+def extend_tables_reference(block_table, held, free_pages, free_used, ctx_lens, q_start, parents, rows, page_size, mask_words,
+                            cp_size, cp_rank, interleave):
+    """Token by token; updates ``block_table``, ``held`` and ``free_used`` in place and returns the six tensors of a plan."""
+    slots = torch.full((rows,), -1, dtype=torch.int64)
+    positions = torch.zeros(rows, dtype=torch.int32)
+    mask = torch.zeros(rows, mask_words, dtype=torch.int64)
+    seq_lens, draft_lens = torch.zeros_like(ctx_lens), torch.zeros_like(ctx_lens)
+    missing = 0
+    for b, n0 in enumerate(ctx_lens.tolist()):
+        r0, r1 = int(q_start[b]), int(q_start[b + 1])
+        before = local_tokens(n0, cp_size, cp_rank, interleave)
+        after = local_tokens(n0 + r1 - r0, cp_size, cp_rank, interleave)
+        need = -(-after // page_size)
+        while int(held[b]) < need and int(held[b]) < block_table.shape[1] and int(free_used) < free_pages.numel():
+            block_table[b, int(held[b])] = free_pages[int(free_used)]
+            held[b] += 1
+            free_used += 1
+        missing += max(need - int(held[b]), 0)
+        room = int(held[b]) * page_size
+        seq_lens[b] = min(after, room)
+        draft_lens[b] = max(int(seq_lens[b]) - before, 0)
+        paths, depths = [], []
+        for j in range(r1 - r0):
+            pos, up = n0 + j, (j - 1 if parents is None else int(parents[r0 + j]))
+            path, depth = (paths[up], depths[up] + 1) if 0 <= up < j else (0, 0)
+            at = local_tokens(pos, cp_size, cp_rank, interleave)
+            if pos // interleave % cp_size == cp_rank and at < room:
+                slots[r0 + j] = int(block_table[b, at // page_size]) * page_size + at % page_size
+                path |= 1 << (at - before)
+            paths.append(path)
+            depths.append(depth)
+            positions[r0 + j] = n0 + depth
+            for w in range(mask_words):
+                word = path >> (64 * w) & (2 ** 64 - 1)
+                mask[r0 + j, w] = word - 2 ** 64 if word >> 63 else word
+    return slots, positions, seq_lens, draft_lens, mask, torch.tensor([missing], dtype=torch.int32)
+
+
+def append_kv_reference(k, v, k_cache, v_cache, slots, hnd):
+    for row, slot in enumerate(slots.tolist()):
+        page = k_cache.shape[2 if hnd else 1]
+        if 0 <= slot < k_cache.shape[0] * page:
+            for cache, x in ((k_cache, k), (v_cache, v)):
+                at = cache[slot // page]
+                (at[:, slot % page] if hnd else at[slot % page]).copy_(x[row])
