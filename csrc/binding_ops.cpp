@@ -3,7 +3,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <cstdlib>
+#include <limits>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -14,6 +16,7 @@
 #include "fused.h"
 #include "oproj.h"
 #include "tensor_map.h"
+#include "tree_attn.h"
 
 namespace {
 
@@ -230,6 +233,93 @@ std::tuple<torch::Tensor, torch::Tensor> gqa_decode(torch::Tensor q, torch::Tens
   return std::make_tuple(o, lse);
 }
 
+// ---- attention of a tree of drafted tokens ------------------------------------------------------------
+std::tuple<torch::Tensor, torch::Tensor> tree_decode(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
+                                                     torch::Tensor block_table, torch::Tensor seq_lens, torch::Tensor q_start,
+                                                     torch::Tensor draft_lens, torch::Tensor mask, double scale, bool lse_base2, bool hnd,
+                                                     int64_t max_seq_len, int64_t max_q_len) {
+  TORCH_CHECK(q.is_cuda(), "all inputs must be on CUDA");
+  const torch::Device dev = q.device();
+  for (const torch::Tensor* t : {&k_cache, &v_cache, &block_table, &seq_lens, &q_start, &draft_lens, &mask})
+    TORCH_CHECK(t->device() == dev, "all inputs must be on one device");
+  const auto type = q.scalar_type();
+  TORCH_CHECK((type == at::ScalarType::BFloat16 || type == at::ScalarType::Half) && k_cache.scalar_type() == type && v_cache.scalar_type() == type,
+              "q / k_cache / v_cache must all be bfloat16 or all float16");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == 128 && q.stride(2) == 1, "q must be [rows, Hq, 128]");
+  TORCH_CHECK(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() && k_cache.size(3) == 128 && k_cache.stride(3) == 1 && v_cache.stride(3) == 1,
+              "caches must be 4-D with head_dim 128 innermost");
+  const int64_t rows = q.size(0), Hq = q.size(1), B = seq_lens.size(0), pages = k_cache.size(0);
+  const int hd = hnd ? 1 : 2, td = hnd ? 2 : 1;
+  const int64_t Hkv = k_cache.size(hd), page = k_cache.size(td);
+  TORCH_CHECK(Hkv >= 1 && Hq % Hkv == 0 && Hq / Hkv >= 1 && Hq / Hkv <= 128, "query heads must be a multiple of the KV heads, at most 128 times as many");
+  TORCH_CHECK(page > 0 && page % 16 == 0, "page size must be a multiple of 16");
+  for (const torch::Tensor* t : {&seq_lens, &q_start, &draft_lens})
+    TORCH_CHECK(t->scalar_type() == at::ScalarType::Int && t->dim() == 1 && t->is_contiguous(), "seq_lens / q_start / draft_lens must be contiguous 1-D int32");
+  TORCH_CHECK(q_start.size(0) == B + 1 && draft_lens.size(0) == B, "q_start must have one element more than seq_lens, draft_lens as many");
+  TORCH_CHECK(block_table.scalar_type() == at::ScalarType::Int && block_table.dim() == 2 && block_table.size(0) == B &&
+                  (block_table.numel() == 0 || block_table.size(1) == 1 || block_table.stride(1) == 1),
+              "block_table must be int32 [B, max_pages] with the pages of a sequence side by side");
+  TORCH_CHECK(mask.scalar_type() == at::ScalarType::Long && mask.dim() == 2 && mask.size(0) == rows && mask.size(1) <= helix::kTreeMaxWords &&
+                  (mask.size(1) <= 1 || mask.stride(1) == 1),
+              "mask must be int64 [rows, words] with at most ", helix::kTreeMaxWords, " words");
+  TORCH_CHECK(rows <= 0x7fffffff && B <= 0x7fffffff && pages <= 0x7fffffff && page <= 0x7fffffff && block_table.size(1) <= 0x7fffffff,
+              "rows, sequences and pages are counted in 32 bits");
+  TORCH_CHECK(scale > 0 && (float)scale > 0.f && std::isfinite((float)scale), "scale must be positive");
+  TORCH_CHECK(rows == 0 || (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && (rows == 1 || q.stride(0) % 8 == 0) && (Hq == 1 || q.stride(1) % 8 == 0)),
+              "rows of q must start on 16-byte boundaries");
+  c10::cuda::CUDAGuard guard(dev);
+  auto stream = at::cuda::getCurrentCUDAStream();
+  torch::Tensor o = torch::empty({rows, Hq, 128}, q.options());
+  torch::Tensor lse = torch::empty({rows, Hq}, q.options().dtype(torch::kFloat32));
+  if (rows == 0) return std::make_tuple(o, lse);
+  if (pages == 0 || B == 0) {
+    o.zero_();
+    lse.fill_(-std::numeric_limits<float>::infinity());
+    return std::make_tuple(o, lse);
+  }
+  helix::TreeDecodeParams p{};
+  p.box_tok = page % 128 == 0 ? 128 : page % 64 == 0 ? 64 : page % 32 == 0 ? 32 : 16;
+  auto map = [&](const torch::Tensor& c, CUtensorMap* m) {
+    const uint64_t dims[4] = {128, (uint64_t)page, (uint64_t)Hkv, (uint64_t)pages};
+    const uint64_t strides[3] = {(uint64_t)c.stride(td) * 2, (uint64_t)c.stride(hd) * 2, (uint64_t)c.stride(0) * 2};
+    const uint32_t box[4] = {64, (uint32_t)p.box_tok, 1, 1};
+    const char* err = nullptr;
+    TORCH_CHECK(helix::encode_tensor_map(m, type == at::ScalarType::Half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                                         c.data_ptr(), dims, strides, box, helix::TmaSwizzle::k128B, &err),
+                "helix: KV cache tensor map: ", err ? err : "?");
+  };
+  map(k_cache, &p.k_map);
+  map(v_cache, &p.v_map);
+  const int group = (int)(Hq / Hkv), sms = helix::device_sm_count();
+  const int max_q = (int)(max_q_len > 0 ? std::min(max_q_len, rows) : rows), longest = (int)std::min<int64_t>(std::max<int64_t>(max_seq_len, 1), 0x7fffff00);
+  p.tiles = helix::tree_pick_tiles(group, max_q);
+  p.ctas = helix::tree_pick_ctas((int)B, (int)Hkv, group, max_q, longest, sms);
+  ScratchUse sc = scratch_for(dev, true, 0, (int64_t)helix::tree_part_o_floats(p.ctas, p.tiles), (int64_t)helix::tree_part_lse_floats(p.ctas, p.tiles));
+  p.q = reinterpret_cast<const uint16_t*>(q.data_ptr());
+  p.q_sr = q.stride(0); p.q_sh = q.stride(1);
+  p.v = reinterpret_cast<const uint16_t*>(v_cache.data_ptr());
+  p.v_sp = v_cache.stride(0); p.v_st = v_cache.stride(td); p.v_sh = v_cache.stride(hd);
+  p.block_table = block_table.data_ptr<int32_t>();
+  p.bt_stride = block_table.stride(0);
+  p.seq_lens = seq_lens.data_ptr<int32_t>();
+  p.q_start = q_start.data_ptr<int32_t>();
+  p.draft_lens = draft_lens.data_ptr<int32_t>();
+  p.mask = reinterpret_cast<const uint64_t*>(mask.data_ptr<int64_t>());
+  p.mask_stride = mask.stride(0);
+  p.o = reinterpret_cast<uint16_t*>(o.data_ptr());
+  p.lse = lse.data_ptr<float>();
+  p.part_o = sc.set.part_a.data_ptr<float>();
+  p.part_lse = sc.set.part_b.data_ptr<float>();
+  p.error_flag = sc.dev.error_flag.data_ptr<int32_t>();
+  p.rows = (int)rows; p.B = (int)B; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.page_size = (int)page; p.max_pages = (int)block_table.size(1);
+  p.n_pages = (int)pages; p.words = (int)mask.size(1);
+  p.is_bf16 = type == at::ScalarType::BFloat16;
+  p.lse_base2 = lse_base2;
+  p.scale = (float)scale;
+  p.timeout_ns = env_timeout_ns();
+  check_cuda(helix::launch_tree_decode(p, env_pdl(), stream), "tree decode launch");
+  return std::make_tuple(o, lse);
+}
 
 constexpr int kMlaDefaultVariant = 2;   // clusters of two CTAs
 
@@ -606,6 +696,10 @@ void register_compute_ops(torch::Library& m) {
       "gqa_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, float scale, bool "
       "lse_base2, bool hnd, int splits, int max_seq_len, bool kv_stable=False) -> (Tensor, Tensor)",
       &gqa_decode);
+  m.def(
+      "tree_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor q_start, Tensor draft_lens, "
+      "Tensor mask, float scale, bool lse_base2, bool hnd, int max_seq_len, int max_q_len) -> (Tensor, Tensor)",
+      &tree_decode);
   m.def(
       "mla_decode(Tensor q_nope, Tensor q_pe, Tensor ckv, Tensor scales, Tensor kpe, Tensor block_table, Tensor seq_lens, "
       "float scale, bool lse_base2, int ctas, int max_seq_len) -> (Tensor, Tensor)",

@@ -1,0 +1,723 @@
+// Attention of a tree of drafted tokens over the paged cache, head_dim 128, bf16 or fp16.
+//
+// Row (t, h) of a sequence and KV head, t a drafted token and h one of the group's query heads, sees all committed tokens of this
+// rank's shard and those drafted ones whose mask bit is set:
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q . k_j - m),   lse = m + log sum_j p_j
+//
+// A group of 8 heads and 16 drafted tokens fill the 128 rows of one tensor-core tile, so both products run on tcgen05: S = Q K^T with
+// both operands in shared memory, P back into tensor memory over S, O += P V with V as it lies in the cache (MN-major).
+//   * Two streams per CTA keep the tensor cores busy: while one softmax warpgroup (a thread per row) works on its scores, the
+//     other stream's products run.  With more than 128 rows (`tiles` = 2) a stream is a tile of rows and every KV tile serves both;
+//     with up to 128 rows the streams take alternate KV tiles of the same rows, and their sums are joined at the end.
+//   * The KV tiles of all (sequence, row tile, KV head) units form one line that is cut into equal shares, a CTA per SM.  A unit that
+//     does not lie inside one share is left in pieces (normalised rows and their LSE), which a second kernel folds.
+//   * The mask only concerns tiles that reach behind the committed tokens: there a row's mask words are shifted into place.
+//     Masked scores are selected away, V rows behind the sequence are cleared in shared memory, and V elements of drafted tokens that are
+//     not finite are cleared too and added at the end to the rows that see them, because 0 * inf would reach all rows.
+//   * P is rounded to the inputs' type for the tensor cores, half a step per probability, which averages out over a row;
+//     maxima, sums and O stay in fp32.  For fp16 P is held 2^7 larger, so that probabilities down to 2^-31 of the largest count.
+// Every mbarrier wait is bounded; on expiry the kernel raises the error flag and leaves.
+#include "tree_attn.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "helix_common.cuh"
+#include "sm100.cuh"
+
+namespace helix {
+namespace {
+
+using namespace sm100;
+
+constexpr int kD = 128, kTile = 128, kRows = 128;
+constexpr int kSlotBytes = kTile * kD * 2;             // 32768: one K or V tile, two halves of [128 tokens x 64 dims]
+constexpr int kHalf = kTile * 128;                     // 16384
+constexpr int kSmWarps = 8, kMmaWarp = 8, kFirstLoad = 9, kLoadWarps = 3, kThreads = 384;
+constexpr int kSlots1 = 6, kSlots2 = 5;                // beside one / two tiles of Q
+constexpr int kMaxSlots = 6;
+constexpr int kSmem = 7 * kSlotBytes + 1024;
+constexpr uint32_t kColS = 0, kColO = 256;             // S0, S1, O0, O1: 128 columns each; P lies over its S
+constexpr int kSeqTable = 512;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kRescale = 8.f;                        // the running maximum moves when a row's grew by more than 2^8
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(uint16_t x) {
+  constexpr uint16_t e = BF16 ? 0x7f80 : 0x7c00;
+  return (x & e) == e;
+}
+template <bool BF16>
+__device__ __forceinline__ float widen(uint16_t x) {
+  return BF16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
+}
+__device__ __forceinline__ void bar_sync_named(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+__device__ __forceinline__ int bar_or_named(int id, int n, int pred) {
+  int r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.s32 p, %3, 0;\n"
+      "bar.red.or.pred q, %1, %2, p;\n"
+      "selp.s32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"(id), "r"(n), "r"(pred)
+      : "memory");
+  return r;
+}
+
+__device__ __forceinline__ int seq_len_of(const TreeDecodeParams& p, int b) {
+  return (int)min((long long)max(p.seq_lens[b], 0), (long long)p.max_pages * p.page_size);
+}
+__device__ __forceinline__ int row0_of(const TreeDecodeParams& p, int b) { return min(max(p.q_start[b], 0), p.rows); }
+
+// One unit: KV tiles of (sequence, tile group of rows, KV head).  A segment is the part of a unit inside this CTA's share.
+struct Segment {
+  int b, kvh, rg;
+  int len, row0, n_rows;       // tokens; first row of the sequence's new tokens; rows of this unit (tokens * group, behind rg's start)
+  int n_tiles, t_begin, count;
+};
+
+struct Walk {
+  long long gcur, g1, base;
+  int b;
+  // tiles of all units of a sequence
+  static __device__ __forceinline__ long long span(const TreeDecodeParams& p, int b) {
+    const int len = seq_len_of(p, b), t = max(row0_of(p, b + 1) - row0_of(p, b), 0);
+    const int per = kRows * p.tiles, group = p.Hq / p.Hkv;
+    return (long long)((len + kTile - 1) / kTile) * (int)(((long long)t * group + per - 1) / per) * p.Hkv;
+  }
+  __device__ __forceinline__ bool next(const TreeDecodeParams& p, Segment& s) {
+    while (gcur < g1 && b < p.B) {
+      const long long n = span(p, b);
+      if (gcur >= base + n) {
+        base += n;
+        ++b;
+        continue;
+      }
+      s.b = b;
+      s.len = seq_len_of(p, b);
+      s.row0 = row0_of(p, b);
+      s.n_tiles = (s.len + kTile - 1) / kTile;
+      const long long off = gcur - base, unit = off / s.n_tiles;
+      s.t_begin = (int)(off - unit * s.n_tiles);
+      s.rg = (int)(unit / p.Hkv);
+      s.kvh = (int)(unit % p.Hkv);
+      s.n_rows = (row0_of(p, b + 1) - s.row0) * (p.Hq / p.Hkv) - s.rg * kRows * p.tiles;
+      s.count = (int)min((long long)(s.n_tiles - s.t_begin), g1 - gcur);
+      gcur += s.count;
+      return true;
+    }
+    return false;
+  }
+};
+
+// 32 visibility bits from drafted token `off` on (negative: committed ones before the first) of a row's mask words
+__device__ __forceinline__ uint32_t mask_bits(const uint64_t* words, int n_words, int off) {
+  if (off <= -32) return 0xffffffffu;
+  auto at = [&](int w) { return w >= 0 && w < 2 * n_words ? reinterpret_cast<const uint32_t*>(words)[w] : 0u; };
+  if (off < 0) return (n_words > 0 ? at(0) << -off : 0u) | (0xffffffffu >> (32 + off));
+  const int w = off >> 5, sh = off & 31;
+  return sh == 0 ? at(w) : at(w) >> sh | at(w + 1) << (32 - sh);
+}
+
+template <bool BF16, int MT>
+__global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_constant__ TreeDecodeParams p) {
+  constexpr int kSlots = MT == 1 ? kSlots1 : kSlots2;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t kv_full[kMaxSlots], kv_free[kMaxSlots], s_full[2], p_full[2], o_full, q_full, drain;
+  __shared__ uint32_t tmem_slot, s_poison[2 * kTreeMaxWords];
+  __shared__ unsigned long long s_rest;
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + MT * kSlotBytes;          // Q first
+  // the place of Q also holds the table of the start, and what the streams tell each other at the end of a segment
+  long long* s_base = reinterpret_cast<long long*>(smem);            // [kSeqTable] first tile of each sequence on the line
+  float (*s_m)[kRows] = reinterpret_cast<float (*)[kRows]>(smem), (*s_l)[kRows] = s_m + 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = p.Hq / p.Hkv;
+
+  if (tid == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&kv_full[i], kLoadWarps);          // each announces its own bytes
+      mbar_init(&kv_free[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
+    mbar_init(&o_full, 1);
+    mbar_init(&q_full, kSmWarps);
+    mbar_init(&drain, 1);
+    s_rest = 0;
+    mbar_fence_init();
+  }
+  if (tid < 2 * kTreeMaxWords) s_poison[tid] = 0;
+  if (warp == kFirstLoad && lane == 0) {
+    tma_prefetch_desc(&p.k_map);
+    tma_prefetch_desc(&p.v_map);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  const unsigned long long deadline = now_ns() + p.timeout_ns;
+
+  // ---- where the sequences lie on the line ---------------------------------------------------------------
+  const int n_tab = min(p.B, kSeqTable);
+  for (int b = tid; b < p.B; b += kThreads) {
+    const long long n = Walk::span(p, b);
+    if (b < kSeqTable) s_base[b] = n;
+    else if (n) atomicAdd(&s_rest, (unsigned long long)n);
+  }
+  __syncthreads();
+  long long total;
+  {
+    // every warp scans the table, and warp 0 leaves the result there
+    const int run = (n_tab + 31) / 32, lo = min(lane * run, n_tab), hi = min(lo + run, n_tab);
+    long long mine = 0;
+    for (int b = lo; b < hi; ++b) mine += s_base[b];
+    long long end = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long below = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += below;
+    }
+    total = __shfl_sync(0xffffffffu, end, 31);
+    __syncthreads();
+    if (warp == 0) {
+      long long at = end - mine;
+      for (int b = lo; b < hi; ++b) {
+        const long long n = s_base[b];
+        s_base[b] = at;
+        at += n;
+      }
+    }
+    __syncthreads();
+  }
+  const long long in_table = total;
+  total += (long long)s_rest;
+  const long long share = max((total + gridDim.x - 1) / (long long)gridDim.x, 1LL);
+  Walk walk;
+  walk.gcur = (long long)blockIdx.x * share;
+  walk.g1 = min(total, walk.gcur + share);
+  if (walk.gcur < in_table) {
+    int lo = 0, hi = n_tab;                        // the last sequence that starts at or before the share
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (s_base[mid] <= walk.gcur) lo = mid; else hi = mid;
+    }
+    walk.b = lo;
+    walk.base = s_base[lo];
+  } else {
+    walk.b = n_tab;
+    walk.base = in_table;
+  }
+  __syncthreads();                                 // the table's place is Q's from here on
+  Segment seg;
+  bool ok = true;
+  uint32_t gt = 0;                                 // KV tiles this CTA has been through: fixes slots and phases
+
+  if (warp < kSmWarps) {
+    // =========================== softmax ===========================
+    // 2 * 208 + 88 registers per thread of a warpgroup are what the block was launched with, 3 * 168
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int st = warp >> 2;                      // this warpgroup's stream
+    const int quad = warp & 3, row = 32 * quad + lane;
+    const uint32_t tq = tmem + ((uint32_t)(32 * quad) << 16);
+    const uint32_t col_s = kColS + 128 * st, col_o = kColO + 128 * st;
+    constexpr float kBias = BF16 ? 0.f : 7.f;
+    const float sl2 = p.scale * kLog2e;
+    const float2 sl22 = make_float2(sl2, sl2);
+    uint32_t steps = 0, n_seg = 0;                 // of this stream, over all segments
+
+    // rows that no unit covers: those of sequences without a token here, and those behind the last sequence
+    {
+      auto clear = [&](int r0, int r1) {
+        for (int64_t i = (int64_t)r0 * p.Hq * 16 + tid; i < (int64_t)r1 * p.Hq * 16; i += 32 * kSmWarps) {
+          reinterpret_cast<uint4*>(p.o)[i] = make_uint4(0, 0, 0, 0);
+          if (i % 16 == 0) p.lse[i / 16] = -INFINITY;
+        }
+      };
+      for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+        if (seq_len_of(p, b) == 0) clear(row0_of(p, b), row0_of(p, b + 1));
+      for (int r = row0_of(p, p.B) + blockIdx.x; r < p.rows; r += gridDim.x) clear(r, r + 1);
+    }
+
+    while (ok && walk.next(p, seg)) {
+      const int unit_row = (MT == 2 ? kRows * st : 0) + row;         // row of the unit
+      const bool valid = unit_row < seg.n_rows;
+      const int grow = seg.rg * kRows * MT + unit_row, node = grow / group;
+      const int64_t qrow = seg.row0 + node, head = seg.kvh * group + grow - node * group;
+      // ---- Q into shared memory: K-major, 128-byte swizzle, halves of 64 dims ---------------------------------
+      {
+        const int c0 = MT == 1 ? 8 * st : 0, cn = MT == 1 ? 8 : 16;
+        uint8_t* dst = smem + (MT == 2 ? st * kSlotBytes : 0);
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + qrow * p.q_sr + head * p.q_sh);
+#pragma unroll
+        for (int c = c0; c < c0 + cn; ++c)
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf + swz128(row, c & 7)) = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full);
+      }
+      const bool warp_valid = __any_sync(0xffffffffu, valid);
+      const int committed = seg.len - min(max(p.draft_lens[seg.b], 0), seg.len);
+      const uint64_t* words = p.mask + (valid ? qrow : 0) * p.mask_stride;
+      float m = -INFINITY, l = 0.f;
+      const int n_steps = MT == 2 ? seg.count : (seg.count - st + 1) / 2;
+
+      for (int k = 0; k < n_steps; ++k, ++steps) {
+        const int i = MT == 2 ? k : 2 * k + st;                      // tile of the segment
+        const int tok0 = (seg.t_begin + i) * kTile;
+        const bool special = tok0 + kTile > committed;               // reaches behind the committed tokens
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[st], steps & 1, deadline));
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (special && (MT == 1 || st == 0)) {
+          // V: rows behind the sequence become zeros, elements of drafted tokens that are not finite too
+          const uint32_t r = 2 * (gt + i) + 1;
+          uint8_t* v = ring + (r % kSlots) * kSlotBytes;
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[r % kSlots], (r / kSlots) & 1, deadline));
+          if (!ok) break;
+          for (int tok = max(committed - tok0, 0) + (row >> 4); tok < kTile; tok += 8) {
+            uint4* at = reinterpret_cast<uint4*>(v + ((row >> 3) & 1) * kHalf + swz128(tok, row & 7));
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (tok0 + tok < seg.len) {
+              x = *at;
+              uint16_t* e = reinterpret_cast<uint16_t*>(&x);
+              bool bad = false;
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (not_finite<BF16>(e[j])) {
+                  e[j] = 0;
+                  bad = true;
+                }
+              if (!bad) continue;
+              const int d = tok0 + tok - committed;
+              if (d < 64 * kTreeMaxWords) atomicOr(&s_poison[d >> 5], 1u << (d & 31));
+            }
+            *at = x;
+          }
+          fence_proxy_async_smem();
+        }
+        if (warp_valid) {
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
+          tmem_ld_wait();
+          if (special) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t seen = mask_bits(words, p.words, tok0 + 32 * c - committed);
+              const int left = seg.len - tok0 - 32 * c;
+              if (left < 32) seen &= left <= 0 ? 0u : (1u << left) - 1u;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if ((seen >> j & 1u) == 0) v[c][j] = 0xff800000u;                // -inf
+            }
+          }
+          float mx[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
+#pragma unroll
+          for (int j = 2; j < 32; j += 2)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])));
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2 - kBias;
+          float alpha = 1.f;
+          if (top > m + kRescale || m == -INFINITY) {
+            const float m_new = fmaxf(m, top);
+            alpha = m == m_new ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - m_new);
+            l *= alpha;
+            m = m_new;
+          }
+          if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            // the scores' commit covers the P V before them: O is complete
+            for (int c0 = 0; c0 < kD; c0 += 16) {
+              uint32_t x[16];
+              tmem_ld_32x32b_x16(tq + col_o + c0, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
+              tmem_st_x16(tq + col_o + c0, x);
+            }
+          }
+          const float mn = m == -INFINITY ? 0.f : -m;
+          const float2 mn2 = make_float2(mn, mn);
+          // m is a rounded product, so s * sl2 - m is off by the rounding, alike for the whole row: up to 2^24 a factor of two at most.
+          // Beyond, the products are rounded too, or the factor could overflow.
+          float2 f2 = sl22;
+          if (__any_sync(0xffffffffu, fabsf(mn) > 16777216.f)) {
+            f2 = make_float2(1.f, 1.f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[c][j] = __float_as_uint(__uint_as_float(v[c][j]) * sl2);
+          }
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 d = fma2(make_float2(__uint_as_float(v[c][2 * j]), __uint_as_float(v[c][2 * j + 1])), f2, mn2);
+              const float2 e = make_float2(fast_exp2(d.x), fast_exp2(d.y));
+              sum = add2(sum, e);
+              pk[j] = pack2<BF16>(e.x, e.y);
+            }
+            tmem_st_x16(tq + col_s + 16 * c, pk);
+          }
+          l += sum.x + sum.y;
+          tmem_st_wait();
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[st]);
+      }
+
+      // ---- O of the segment: join the streams, normalise, write the result or a piece ----------------------
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full, n_seg & 1, deadline));
+      ++n_seg;
+      s_m[st][row] = m;
+      s_l[st][row] = l;
+      bar_sync_named(1, 32 * kSmWarps);
+      tc_fence_after_sync();
+      const bool both = MT == 1 && seg.count > 1;
+      float f0 = 1.f, f1 = 0.f, M = m, L = l;
+      if (MT == 1) {
+        const float m0 = s_m[0][row], m1 = both ? s_m[1][row] : -INFINITY;
+        M = fmaxf(m0, m1);
+        f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - M);
+        f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - M);
+        L = s_l[0][row] * f0 + (both ? s_l[1][row] * f1 : 0.f);
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;                    // a NaN stays one
+      f0 *= inv;
+      f1 *= inv;
+      uint32_t poisoned = 0;
+#pragma unroll
+      for (int w = 0; w < 2 * kTreeMaxWords; ++w) poisoned |= s_poison[w];
+      const bool whole = seg.count == seg.n_tiles;
+      // slot 1: the piece that starts its unit; a CTA has at most one of each kind
+      const int64_t piece = ((int64_t)blockIdx.x * 2 + (seg.t_begin == 0 ? 1 : 0)) * kRows * MT + unit_row;
+      const int c_begin = MT == 1 ? 64 * st : 0, c_end = MT == 1 ? c_begin + 64 : kD;
+      if (warp_valid) {
+        for (int c0 = c_begin; c0 < c_end; c0 += 16) {
+          uint32_t x[16], y[16];
+          tmem_ld_32x32b_x16(tq + (MT == 1 ? kColO : col_o) + c0, x);
+          if (both) tmem_ld_32x32b_x16(tq + kColO + 128 + c0, y);
+          tmem_ld_wait();
+          float o[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            o[j] = f0 == 0.f ? 0.f : __uint_as_float(x[j]) * f0;
+            if (both && f1 != 0.f) o[j] += __uint_as_float(y[j]) * f1;
+          }
+          if (poisoned != 0 && valid) {
+            for (int d = 0; d < 64 * p.words; ++d) {
+              const int tok = committed + d;
+              if ((s_poison[d >> 5] >> (d & 31) & 1u) == 0 || (words[d >> 6] >> (d & 63) & 1u) == 0 || tok >= seg.len) continue;
+              const int pg = p.block_table[seg.b * p.bt_stride + tok / p.page_size];
+              if (pg < 0 || pg >= p.n_pages) continue;
+              const uint16_t* src = p.v + pg * p.v_sp + (tok % p.page_size) * p.v_st + seg.kvh * p.v_sh + c0;
+              for (int j = 0; j < 16; ++j)
+                if (not_finite<BF16>(src[j])) o[j] += widen<BF16>(src[j]);
+            }
+          }
+          if (!valid) continue;
+          if (whole) {
+            uint4* dst = reinterpret_cast<uint4*>(p.o + (qrow * p.Hq + head) * kD + c0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              dst[j] = make_uint4(pack2<BF16>(o[8 * j], o[8 * j + 1]), pack2<BF16>(o[8 * j + 2], o[8 * j + 3]),
+                                  pack2<BF16>(o[8 * j + 4], o[8 * j + 5]), pack2<BF16>(o[8 * j + 6], o[8 * j + 7]));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + piece * kD + c0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
+        }
+        if (valid && (MT == 2 || st == 0)) {
+          const float lse2 = L == 0.f ? -INFINITY : M + log2f(L);
+          if (whole) p.lse[qrow * p.Hq + head] = p.lse_base2 ? lse2 : lse2 * kLn2;
+          else p.part_lse[piece] = lse2;
+        }
+      }
+      tc_fence_before_sync();
+      // O, s_m, s_l and s_poison are free; a warp that gave up takes the others with it, or they would wait for it
+      if (bar_or_named(1, 32 * kSmWarps, ok ? 0 : 1)) ok = false;
+      if (poisoned != 0 && tid < 2 * kTreeMaxWords) s_poison[tid] = 0;
+      gt += seg.count;
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
+  if (warp >= kFirstLoad) {
+    // =========================== loads ===========================
+    // Boxes of 16 tokens x 64 dims (a page of 16 tokens allows no larger ones): 32 per tile, shared by three warps, each issued by
+    // one elected lane of a warp that has stayed together.  One warp whose lanes issued a box each took ~136 cycles per box,
+    // 4400 per tile, which bounded everything (64 x 8192 tokens 528 us).
+    const int per_tile = kTile / p.box_tok, lw = warp - kFirstLoad;
+    uint32_t issued = 0;
+    while (ok && walk.next(p, seg)) {
+      const int32_t* bt = p.block_table + (int64_t)seg.b * p.bt_stride;
+      auto page_at = [&](int i) {                  // page of block `lane` in tile i of the segment
+        const int tok = (seg.t_begin + i) * kTile + lane * p.box_tok;
+        return i < seg.count && lane < per_tile && tok < seg.len ? __ldg(bt + tok / p.page_size) : 0;
+      };
+      int page = page_at(0);
+      for (int i = 0; i < seg.count && ok; ++i) {
+        const int tok0 = (seg.t_begin + i) * kTile, in_page = (tok0 + lane * p.box_tok) % p.page_size;
+        const int boxes = 2 * ((min(seg.len - tok0, kTile) + p.box_tok - 1) / p.box_tok);
+        const int mine = (boxes - lw + kLoadWarps - 1) / kLoadWarps;
+        const int next = page_at(i + 1);
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t r = 2 * (gt + i) + kv, slot = r % kSlots;
+          if (r >= (uint32_t)kSlots) ok = __all_sync(0xffffffffu, mbar_wait(&kv_free[slot], (r / kSlots - 1) & 1, deadline));
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(&kv_full[slot], (uint32_t)mine * p.box_tok * kD);
+          __syncwarp();
+          for (int j = lw; j < boxes; j += kLoadWarps) {
+            const int pg = __shfl_sync(0xffffffffu, page, j >> 1), at = __shfl_sync(0xffffffffu, in_page, j >> 1), half = j & 1;
+            if (elect_one())
+              tma_load_4d(ring + slot * kSlotBytes + half * kHalf + (j >> 1) * p.box_tok * 128, kv == 0 ? &p.k_map : &p.v_map,
+                          &kv_full[slot], 64 * half, at, seg.kvh, pg);
+            __syncwarp();
+          }
+          issued = r + 1;
+        }
+        page = next;
+      }
+      gt += seg.count;
+    }
+    if (!ok) {
+      // nothing may land in this CTA's shared memory after it has left
+      const unsigned long long limit = now_ns() + 10000000ull;
+      for (uint32_t r = issued > (uint32_t)kSlots ? issued - kSlots : 0; r < issued; ++r) mbar_wait(&kv_full[r % kSlots], (r / kSlots) & 1, limit);
+    }
+  } else if (warp == kMmaWarp) {
+    // =========================== MMA issue ===========================
+    constexpr uint32_t fmt = BF16 ? umma_idesc_bf16(kRows, kTile) : umma_idesc_bf16(kRows, kTile) & ~((1u << 7) | (1u << 10));
+    constexpr uint32_t id_s = fmt, id_o = fmt | (1u << 16);          // V is MN-major
+    // all 512 columns are this CTA's: tensor memory starts at column 0, and no register holds the base
+    const uint64_t d_q = umma_desc_k_sw128(smem_u32(smem)), d_k = umma_desc_k_sw128(smem_u32(ring)),
+                   d_v = umma_desc_mn_sw128(smem_u32(ring), kHalf);
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0; };
+    uint32_t steps[2] = {0, 0}, n_seg = 0;
+    auto scores = [&](int s, int i_lane, bool last_user) {           // S of stream s from tile i
+      const uint32_t r = 2 * (gt + __shfl_sync(0xffffffffu, i_lane, 0)), slot = r % kSlots;
+      if (!wait(&kv_full[slot], (r / kSlots) & 1)) return false;
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint32_t kb = slot * kSlotBytes, qb = MT == 2 ? s * kSlotBytes : 0;
+#pragma unroll
+        for (int ks = 0; ks < kD / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
+          umma_bf16(kColS + 128 * s, d_q + ((qb + off) >> 4), d_k + ((kb + off) >> 4), id_s, ks > 0);
+        }
+        umma_commit(&s_full[s]);
+        if (last_user) umma_commit(&kv_free[slot]);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto values = [&](int s, int i_lane, bool first, bool last_user) {   // O of stream s += P V of tile i
+      const uint32_t r = 2 * (gt + __shfl_sync(0xffffffffu, i_lane, 0)) + 1, slot = r % kSlots;
+      if (!wait(&p_full[s], steps[s] & 1) || !wait(&kv_full[slot], (r / kSlots) & 1)) return false;
+      ++steps[s];
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint32_t vb = slot * kSlotBytes;
+#pragma unroll
+        for (int ks = 0; ks < kTile / 16; ++ks) {
+          const uint32_t lo = (uint32_t)d_v + ((vb + ks * 2048) >> 4);
+          if (ks == 0) umma_bf16_ts_first(kColO + 128 * s, kColS + 128 * s, lo, (uint32_t)(d_v >> 32), id_o, first ? 0u : 1u);
+          else umma_bf16_ts(kColO + 128 * s, kColS + 128 * s + 8 * ks, lo, (uint32_t)(d_v >> 32), id_o);
+        }
+        if (last_user) umma_commit(&kv_free[slot]);
+      }
+      __syncwarp();
+      return true;
+    };
+    while (ok && walk.next(p, seg)) {
+      ok = wait(&q_full, n_seg & 1);
+      ++n_seg;
+      if (!ok) break;
+      tc_fence_after_sync();
+      const int n0 = MT == 2 ? seg.count : (seg.count + 1) / 2, n1 = MT == 2 ? seg.count : seg.count / 2;
+      auto tile = [&](int s, int k) { return MT == 2 ? k : 2 * k + s; };
+      ok = scores(0, tile(0, 0), MT == 1);
+      if (ok && n1 > 0) ok = scores(1, tile(1, 0), true);
+      for (int k = 0; k < n0 && ok; ++k) {
+        ok = values(0, tile(0, k), k == 0, MT == 1);
+        if (ok && k + 1 < n0) ok = scores(0, tile(0, k + 1), MT == 1);
+        if (ok && k < n1) ok = values(1, tile(1, k), k == 0, true);
+        if (ok && k + 1 < n1) ok = scores(1, tile(1, k + 1), true);
+      }
+      if (ok && elect_one()) umma_commit(&o_full);
+      __syncwarp();
+      gt += seg.count;
+    }
+    if (!ok) {
+      if (elect_one()) umma_commit(&drain);        // nothing of this CTA's may be in flight when it leaves
+      mbar_wait(&drain, 0, now_ns() + 10000000ull);
+    }
+  }
+  if (!ok && lane == 0) atomicCAS(p.error_flag, 0, (int)kTimeoutMbarrier);
+
+  // ---- what the fold has to do: the unit that this CTA begins and the next ones finish ---------------------
+  if (tid == 0) {
+    Walk w = walk;                                 // at the end of the share: seg is its last segment
+    int4 note = make_int4(-1, 0, 0, 0);
+    if (w.gcur > (long long)blockIdx.x * share && seg.t_begin == 0 && seg.count < seg.n_tiles)
+      note = make_int4(seg.b, seg.kvh, seg.rg, (int)((w.gcur - seg.count + seg.n_tiles - 1) / share));
+    reinterpret_cast<int4*>(p.part_lse + tree_notes_at(p.ctas, p.tiles))[blockIdx.x] = note;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// The pieces of a unit that several CTAs shared, in the order of the CTAs.  Block (c, y): the unit that CTA c begins, a warp per row.
+constexpr int kFoldThreads = 256, kFoldBatch = 8;
+template <bool BF16>
+__global__ void __launch_bounds__(kFoldThreads) tree_fold_kernel(const __grid_constant__ TreeDecodeParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 note = __ldcg(reinterpret_cast<const int4*>(p.part_lse + tree_notes_at(p.ctas, p.tiles)) + blockIdx.x);
+  if (note.x < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.Hq / p.Hkv, per = kRows * p.tiles;
+  const int row0 = row0_of(p, note.x), n_rows = min((row0_of(p, note.x + 1) - row0) * group - note.z * per, per);
+  const int n = note.w - (int)blockIdx.x + 1;
+  for (int r = blockIdx.y * (kFoldThreads / 32) + warp; r < n_rows; r += gridDim.y * (kFoldThreads / 32)) {
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += kFoldBatch) {
+      float4 v[kFoldBatch];
+      float l[kFoldBatch];
+#pragma unroll
+      for (int j = 0; j < kFoldBatch; ++j) {
+        l[j] = -INFINITY;
+        v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + j < n) {
+          const int64_t piece = (((int64_t)blockIdx.x + i0 + j) * 2 + (i0 + j == 0 ? 1 : 0)) * per + r;
+          l[j] = __ldcg(p.part_lse + piece);
+          v[j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + piece * kD) + lane);
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int j = 0; j < kFoldBatch; ++j) top = fmaxf(top, l[j]);
+      const float keep = M == -INFINITY ? 0.f : fast_exp2(M - top);
+      M = top;
+      L *= keep;
+      acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+      for (int j = 0; j < kFoldBatch; ++j) {
+        if (l[j] == -INFINITY) continue;
+        const float w = fast_exp2(l[j] - top);
+        L += w;
+        acc.x += w * v[j].x;
+        acc.y += w * v[j].y;
+        acc.z += w * v[j].z;
+        acc.w += w * v[j].w;
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int grow = note.z * per + r, node = grow / group;
+    const int64_t at = (int64_t)(row0 + node) * p.Hq + note.y * group + grow - node * group;
+    *(reinterpret_cast<uint2*>(p.o + at * kD) + lane) = make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+    if (lane == 0) {
+      const float lse2 = L == 0.f ? -INFINITY : M + log2f(L);
+      p.lse[at] = p.lse_base2 ? lse2 : lse2 * kLn2;
+    }
+  }
+}
+
+using Fn = void (*)(TreeDecodeParams);
+
+}  // namespace
+
+int tree_pick_tiles(int group, int max_q) { return (long long)group * max_q > kRows ? 2 : 1; }
+
+int tree_pick_ctas(int B, int Hkv, int group, int max_q, int max_seq_len, int sm_count) {
+  const long long per = (long long)kRows * tree_pick_tiles(group, max_q);
+  const long long tiles = (long long)std::max(B, 1) * Hkv * (((long long)group * std::max(max_q, 1) + per - 1) / per) *
+                          std::max((max_seq_len + kTile - 1) / kTile, 1);
+  return (int)std::min<long long>(tiles, sm_count);
+}
+
+cudaError_t launch_tree_decode(const TreeDecodeParams& p, bool pdl, cudaStream_t stream) {
+  if (p.rows <= 0) return cudaSuccess;
+  if (p.Hkv <= 0 || p.Hq % p.Hkv != 0 || p.tiles < 1 || p.tiles > 2 || p.ctas < 1 || p.words < 0 || p.words > kTreeMaxWords ||
+      (p.box_tok != 16 && p.box_tok != 32 && p.box_tok != 64 && p.box_tok != 128) || p.page_size % p.box_tok != 0)
+    return cudaErrorInvalidValue;
+  Fn fn = p.is_bf16 ? (p.tiles == 1 ? (Fn)tree_decode_kernel<true, 1> : (Fn)tree_decode_kernel<true, 2>)
+                    : (p.tiles == 1 ? (Fn)tree_decode_kernel<false, 1> : (Fn)tree_decode_kernel<false, 2>);
+  static bool attr_set[64][4] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int which = (p.is_bf16 ? 2 : 0) + p.tiles - 1;
+  cudaError_t e = cudaSuccess;
+  if (dev >= 64 || !attr_set[dev][which]) {
+    e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_set[dev][which] = true;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.ctas, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, fn, p);
+  if (e != cudaSuccess) return e;
+  // the fold is always chained to this launch; it waits for the whole grid before it reads a piece
+  cfg.gridDim = dim3(p.ctas, 8, 1);
+  cfg.blockDim = dim3(kFoldThreads, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, p.is_bf16 ? (Fn)tree_fold_kernel<true> : (Fn)tree_fold_kernel<false>, p);
+}
+
+}  // namespace helix

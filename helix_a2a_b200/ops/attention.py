@@ -42,6 +42,36 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
                                  layout == "HND", splits, max_seq_len, kv_stable)
 
 
+def tree_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                seq_lens: torch.Tensor, q_start: torch.Tensor, draft_lens: torch.Tensor, mask: torch.Tensor, *,
+                scale: Optional[float] = None, lse_base2: bool = False, layout: str = "HND", max_seq_len: int = 0,
+                max_q_len: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention of several drafted tokens per sequence over its local KV pages, masked by their tree.
+
+    ``q [rows, Hq, 128]``, bf16 or fp16 like the caches (laid out as for :func:`gqa_decode`): rows ``q_start[b]`` to
+    ``q_start[b + 1]`` belong to sequence ``b``.  ``seq_lens [B]`` counts the tokens of the LOCAL shard, whose last
+    ``draft_lens [B]`` are the step's own; ``mask [rows, words]`` (int64, up to 4 words) has a bit for each of these: a row sees every
+    token before them, and the ``i``-th of them if bit ``i`` is set (those past the mask's bits are not seen).
+    :func:`helix_a2a_b200.ops.paged.extend_tables` makes the last four arguments.  Masked tokens do not reach a row whatever they
+    hold.  Returns what the exchange takes, ``o [rows, Hq, 128]`` and ``lse [rows, Hq]`` (fp32, natural log or base 2); a row that sees
+    nothing, as rows behind ``q_start[B]`` do, is zero with LSE ``-inf``.
+
+    ``max_seq_len`` and ``max_q_len`` (0: unknown) only help to divide the work; results hold for any lengths.
+    """
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    if layout not in ("HND", "NHD"):
+        raise ValueError("layout must be 'HND' or 'NHD'")
+    if not q.is_cuda:
+        kc = k_cache if layout == "HND" else k_cache.permute(0, 2, 1, 3)
+        vc = v_cache if layout == "HND" else v_cache.permute(0, 2, 1, 3)
+        o, lse = rm.tree_decode_reference(q, kc, vc, block_table, seq_lens, q_start, draft_lens, mask, scale, lse_base2)
+        return o.to(q.dtype), lse
+    if max_seq_len <= 0:
+        max_seq_len = block_table.shape[1] * (k_cache.shape[2] if layout == "HND" else k_cache.shape[1])
+    return _ext.ops().tree_decode(q, k_cache, v_cache, block_table, seq_lens, q_start, draft_lens, mask, float(scale), lse_base2,
+                                  layout == "HND", max_seq_len, max_q_len)
+
+
 def mla_decode(q_nope: torch.Tensor, q_pe: torch.Tensor, ckv_fp8: torch.Tensor, scales: torch.Tensor,
                kpe: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, *, scale: float,
                lse_base2: bool = False, ctas: int = 0, max_seq_len: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:

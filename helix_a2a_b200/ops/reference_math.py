@@ -281,3 +281,17 @@ def append_kv_reference(k, v, k_cache, v_cache, slots, hnd):
             for cache, x in ((k_cache, k), (v_cache, v)):
                 at = cache[slot // page]
                 (at[:, slot % page] if hnd else at[slot % page]).copy_(x[row])
+
+
+def tree_decode_reference(q, k_cache, v_cache, block_table, seq_lens, q_start, draft_lens, mask, scale, base2=False):
+    """Row by row: ``q [rows, H, D]`` over the tokens its mask lets it see.  Returns fp32 ``o [rows, H, D]`` and ``lse [rows, H]``."""
+    rows, H, D = q.shape
+    o = torch.zeros(rows, H, D)
+    lse = torch.full((rows, H), float("-inf"))
+    for b in range(seq_lens.numel()):
+        n, d = int(seq_lens[b]), int(draft_lens[b])
+        k, v = gather_paged_kv(k_cache, block_table[b], n), gather_paged_kv(v_cache, block_table[b], n)
+        for r in range(int(q_start[b]), int(q_start[b + 1])):
+            seen = [i for i in range(n - d)] + [n - d + i for i in range(min(d, 64 * mask.shape[1])) if int(mask[r, i // 64]) >> (i % 64) & 1]
+            o[r], lse[r] = (t[0] for t in partial_attention(q[r:r + 1], k[seen], v[seen], scale, base2))
+    return o, lse
