@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0; };
     uint32_t steps[2] = {0, 0}, n_seg = 0;
     auto scores = [&](int s, int i_lane, bool last_user) {           // S of stream s from tile i
-      const uint32_t r = 2 * (gt + __shfl_sync(0xffffffffu, i_lane, 0)), slot = r % kSlots;
+      const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0), slot = r % kSlots;
       if (!wait(&kv_full[slot], (r / kSlots) & 1)) return false;
       tc_fence_after_sync();
       if (elect_one()) {
@@ -554,8 +554,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       __syncwarp();
       return true;
     };
-    auto values = [&](int s, int i_lane, bool first, bool last_user) {   // O of stream s += P V of tile i
-      const uint32_t r = 2 * (gt + __shfl_sync(0xffffffffu, i_lane, 0)) + 1, slot = r % kSlots;
+    auto values = [&](int s, int i_lane, int k_lane, bool last_user) {   // O of stream s += P V of tile i
+      const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0) + 1, later = __shfl_sync(0xffffffffu, k_lane, 0), slot = r % kSlots;
       if (!wait(&p_full[s], steps[s] & 1) || !wait(&kv_full[slot], (r / kSlots) & 1)) return false;
       ++steps[s];
       tc_fence_after_sync();
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
 #pragma unroll
         for (int ks = 0; ks < kTile / 16; ++ks) {
           const uint32_t lo = (uint32_t)d_v + ((vb + ks * 2048) >> 4);
-          if (ks == 0) umma_bf16_ts_first(kColO + 128 * s, kColS + 128 * s, lo, (uint32_t)(d_v >> 32), id_o, first ? 0u : 1u);
+          if (ks == 0) umma_bf16_ts_first(kColO + 128 * s, kColS + 128 * s, lo, (uint32_t)(d_v >> 32), id_o, later);
           else umma_bf16_ts(kColO + 128 * s, kColS + 128 * s + 8 * ks, lo, (uint32_t)(d_v >> 32), id_o);
         }
         if (last_user) umma_commit(&kv_free[slot]);
@@ -582,9 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       ok = scores(0, tile(0, 0), MT == 1);
       if (ok && n1 > 0) ok = scores(1, tile(1, 0), true);
       for (int k = 0; k < n0 && ok; ++k) {
-        ok = values(0, tile(0, k), k == 0, MT == 1);
+        ok = values(0, tile(0, k), k, MT == 1);
         if (ok && k + 1 < n0) ok = scores(0, tile(0, k + 1), MT == 1);
-        if (ok && k < n1) ok = values(1, tile(1, k), k == 0, true);
+        if (ok && k < n1) ok = values(1, tile(1, k), k, true);
         if (ok && k + 1 < n1) ok = scores(1, tile(1, k + 1), true);
       }
       if (ok && elect_one()) umma_commit(&o_full);
