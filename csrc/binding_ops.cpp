@@ -264,6 +264,8 @@ std::tuple<torch::Tensor, torch::Tensor> tree_decode(torch::Tensor q, torch::Ten
               "mask must be int64 [rows, words] with at most ", helix::kTreeMaxWords, " words");
   TORCH_CHECK(rows <= 0x7fffffff && B <= 0x7fffffff && pages <= 0x7fffffff && page <= 0x7fffffff && block_table.size(1) <= 0x7fffffff,
               "rows, sequences and pages are counted in 32 bits");
+  TORCH_CHECK(rows * (Hq / Hkv) <= 0x7fffffff && helix::tree_line_bound(rows, B, Hkv, Hq / Hkv, block_table.size(1) * page) <= 0x7fffffff,
+              "rows, KV heads and table width are too large for one call");
   TORCH_CHECK(scale > 0 && (float)scale > 0.f && std::isfinite((float)scale), "scale must be positive");
   TORCH_CHECK(rows == 0 || (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && (rows == 1 || q.stride(0) % 8 == 0) && (Hq == 1 || q.stride(1) % 8 == 0)),
               "rows of q must start on 16-byte boundaries");
@@ -292,9 +294,12 @@ std::tuple<torch::Tensor, torch::Tensor> tree_decode(torch::Tensor q, torch::Ten
   map(v_cache, &p.v_map);
   const int group = (int)(Hq / Hkv), sms = helix::device_sm_count();
   const int max_q = (int)(max_q_len > 0 ? std::min(max_q_len, rows) : rows), longest = (int)std::min<int64_t>(std::max<int64_t>(max_seq_len, 1), 0x7fffff00);
-  p.tiles = helix::tree_pick_tiles(group, max_q);
-  p.ctas = helix::tree_pick_ctas((int)B, (int)Hkv, group, max_q, longest, sms);
-  ScratchUse sc = scratch_for(dev, true, 0, (int64_t)helix::tree_part_o_floats(p.ctas, p.tiles), (int64_t)helix::tree_part_lse_floats(p.ctas, p.tiles));
+  const helix::TreePlan plan = helix::tree_plan((int)B, (int)Hkv, group, max_q, longest, sms);
+  p.tiles = plan.tiles;
+  p.ctas = plan.ctas;
+  p.whole = plan.whole;
+  ScratchUse sc = scratch_for(dev, !p.whole, 0, p.whole ? 0 : (int64_t)helix::tree_part_o_floats(p.ctas, p.tiles),
+                              p.whole ? 0 : (int64_t)helix::tree_part_lse_floats(p.ctas, p.tiles));
   p.q = reinterpret_cast<const uint16_t*>(q.data_ptr());
   p.q_sr = q.stride(0); p.q_sh = q.stride(1);
   p.v = reinterpret_cast<const uint16_t*>(v_cache.data_ptr());
@@ -308,8 +313,8 @@ std::tuple<torch::Tensor, torch::Tensor> tree_decode(torch::Tensor q, torch::Ten
   p.mask_stride = mask.stride(0);
   p.o = reinterpret_cast<uint16_t*>(o.data_ptr());
   p.lse = lse.data_ptr<float>();
-  p.part_o = sc.set.part_a.data_ptr<float>();
-  p.part_lse = sc.set.part_b.data_ptr<float>();
+  p.part_o = p.whole ? nullptr : sc.set.part_a.data_ptr<float>();
+  p.part_lse = p.whole ? nullptr : sc.set.part_b.data_ptr<float>();
   p.error_flag = sc.dev.error_flag.data_ptr<int32_t>();
   p.rows = (int)rows; p.B = (int)B; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.page_size = (int)page; p.max_pages = (int)block_table.size(1);
   p.n_pages = (int)pages; p.words = (int)mask.size(1);

@@ -37,11 +37,13 @@ constexpr int kD = 128, kTile = 128, kRows = 128;
 constexpr int kSlotBytes = kTile * kD * 2;             // 32768: one K or V tile, two halves of [128 tokens x 64 dims]
 constexpr int kHalf = kTile * 128;                     // 16384
 constexpr int kSmWarps = 8, kMmaWarp = 8, kFirstLoad = 9, kLoadWarps = 3, kThreads = 384;
-constexpr int kSlots1 = 6, kSlots2 = 5;                // beside one / two tiles of Q
-constexpr int kMaxSlots = 6;
-constexpr int kSmem = 7 * kSlotBytes + 1024;
+constexpr int kSlots = 5;                              // beside two tiles of Q
+constexpr int kSmem = (2 + kSlots) * kSlotBytes + 1024;
 constexpr uint32_t kColS = 0, kColO = 256;             // S0, S1, O0, O1: 128 columns each; P lies over its S
 constexpr int kSeqTable = 512;
+constexpr int kWholeTiles = 4;                         // units of up to so many tiles stay whole, a CTA each
+constexpr int kUnitCost = 2;                           // what a unit costs besides its tiles, in tiles
+constexpr int kPolyOf8 = 3;                            // of 8 pairs of exponentials, how many the FMA pipe computes
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;                        // the running maximum moves when a row's grew by more than 2^8
 
@@ -56,6 +58,38 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=l"(r)
       : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
   return *reinterpret_cast<float2*>(&r);
+}
+// 2^x for two numbers up to 127, on the FMA pipe: 2^n times a polynomial in f = x - n, |f| <= 1/2, which is 2^f to 1.5e-5 (equal
+// error at all extrema, 1 at f = 0), far below the step of bf16 and fp16 that P is rounded to.  Below 2^-126 comes exactly 0.
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), neg = make_float2(-12582912.f, -12582912.f);     // 1.5 * 2^23
+  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 t = add2(x, magic), n = add2(t, neg), f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 r = make_float2(0x1.564e84p-7f, 0x1.564e84p-7f);
+  r = fma2(r, f, make_float2(0x1.cc088cp-5f, 0x1.cc088cp-5f));
+  r = fma2(r, f, make_float2(0x1.eba26ap-3f, 0x1.eba26ap-3f));
+  r = fma2(r, f, make_float2(0x1.62da5ap-1f, 0x1.62da5ap-1f));
+  r = fma2(r, f, make_float2(1.f, 1.f));
+  r = make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
+                  __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
+  return add2(r, make_float2(-0x1p-126f, -0x1p-126f));
+}
+// maxima that pass a NaN on
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 32 bytes, a whole sector
+__device__ __forceinline__ void st_global_x8(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -97,42 +131,47 @@ __device__ __forceinline__ int seq_len_of(const TreeDecodeParams& p, int b) {
 }
 __device__ __forceinline__ int row0_of(const TreeDecodeParams& p, int b) { return min(max(p.q_start[b], 0), p.rows); }
 
-// One unit: KV tiles of (sequence, tile group of rows, KV head).  A segment is the part of a unit inside this CTA's share.
+// One unit: the KV tiles of (sequence, tile group of rows, KV head).  On the line a unit is its tiles behind kUnitCost places that stand
+// for what a unit costs besides (Q, the last tile's way through the pipeline, its output): without them CTAs with many short units
+// were the last by far (24 ragged sequences up to 9000 tokens: 160 us against 85 for the others).  A segment is the part of a unit
+// inside this CTA's share.  With `whole` a CTA takes units blockIdx.x, blockIdx.x + gridDim.x, ... from end to end.
 struct Segment {
   int b, kvh, rg;
   int len, row0, n_rows;       // tokens; first row of the sequence's new tokens; rows of this unit (tokens * group, behind rg's start)
   int n_tiles, t_begin, count;
+  int end;                     // of the unit, on the line
 };
 
 struct Walk {
-  long long gcur, g1, base;
-  int b;
-  // tiles of all units of a sequence
-  static __device__ __forceinline__ long long span(const TreeDecodeParams& p, int b) {
-    const int len = seq_len_of(p, b), t = max(row0_of(p, b + 1) - row0_of(p, b), 0);
-    const int per = kRows * p.tiles, group = p.Hq / p.Hkv;
-    return (long long)((len + kTile - 1) / kTile) * (int)(((long long)t * group + per - 1) / per) * p.Hkv;
+  int gcur, g1, base, b;
+  static __device__ __forceinline__ int units(const TreeDecodeParams& p, int b) {
+    const int per = kRows * p.tiles, t = max(row0_of(p, b + 1) - row0_of(p, b), 0);
+    return seq_len_of(p, b) > 0 ? (int)(((unsigned)t * (unsigned)(p.Hq / p.Hkv) + per - 1) / per) * p.Hkv : 0;
+  }
+  static __device__ __forceinline__ int length(const TreeDecodeParams& p, int b) {     // of a unit
+    return p.whole ? 1 : (seq_len_of(p, b) + kTile - 1) / kTile + kUnitCost;
   }
   __device__ __forceinline__ bool next(const TreeDecodeParams& p, Segment& s) {
     while (gcur < g1 && b < p.B) {
-      const long long n = span(p, b);
+      const int per = length(p, b), n = units(p, b) * per;
       if (gcur >= base + n) {
         base += n;
         ++b;
         continue;
       }
+      const int unit = (gcur - base) / per, at = gcur - base - unit * per, to = min(per, at + g1 - gcur);
       s.b = b;
       s.len = seq_len_of(p, b);
       s.row0 = row0_of(p, b);
       s.n_tiles = (s.len + kTile - 1) / kTile;
-      const long long off = gcur - base, unit = off / s.n_tiles;
-      s.t_begin = (int)(off - unit * s.n_tiles);
-      s.rg = (int)(unit / p.Hkv);
-      s.kvh = (int)(unit % p.Hkv);
+      s.rg = unit / p.Hkv;
+      s.kvh = unit - s.rg * p.Hkv;
       s.n_rows = (row0_of(p, b + 1) - s.row0) * (p.Hq / p.Hkv) - s.rg * kRows * p.tiles;
-      s.count = (int)min((long long)(s.n_tiles - s.t_begin), g1 - gcur);
-      gcur += s.count;
-      return true;
+      s.t_begin = p.whole ? 0 : max(at - kUnitCost, 0);
+      s.count = p.whole ? s.n_tiles : max(to - kUnitCost, 0) - s.t_begin;
+      s.end = base + (unit + 1) * per;
+      gcur += p.whole ? gridDim.x : to - at;
+      if (s.count > 0) return true;
     }
     return false;
   }
@@ -149,17 +188,15 @@ __device__ __forceinline__ uint32_t mask_bits(const uint64_t* words, int n_words
 
 template <bool BF16, int MT>
 __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_constant__ TreeDecodeParams p) {
-  constexpr int kSlots = MT == 1 ? kSlots1 : kSlots2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t kv_full[kMaxSlots], kv_free[kMaxSlots], s_full[2], p_full[2], o_full, q_full, drain;
-  __shared__ uint32_t tmem_slot, s_poison[2 * kTreeMaxWords];
-  __shared__ unsigned long long s_rest;
+  __shared__ __align__(8) uint64_t kv_full[kSlots], kv_free[kSlots], s_full[2], p_full[2][2], o_full, q_full, drain;
+  __shared__ uint32_t tmem_slot, s_poison[2][2 * kTreeMaxWords];      // by turns: a segment's is cleared behind its end
+  __shared__ float s_x[2][kRows];                  // what the streams tell each other at the end of a segment
+  __shared__ int s_rest;
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + MT * kSlotBytes;          // Q first
-  // the place of Q also holds the table of the start, and what the streams tell each other at the end of a segment
-  long long* s_base = reinterpret_cast<long long*>(smem);            // [kSeqTable] first tile of each sequence on the line
-  float (*s_m)[kRows] = reinterpret_cast<float (*)[kRows]>(smem), (*s_l)[kRows] = s_m + 2;
+  uint8_t* ring = smem + 2 * kSlotBytes;           // behind two tiles of Q: both row tiles, or this segment's and the next one's
+  int* s_base = reinterpret_cast<int*>(smem);      // [kSeqTable] first place of each sequence on the line, until Q comes
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.Hq / p.Hkv;
 
@@ -170,7 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i][0], 4);                 // halves of 64 tokens
+      mbar_init(&p_full[i][1], 4);
     }
     mbar_init(&o_full, 1);
     mbar_init(&q_full, kSmWarps);
@@ -178,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     s_rest = 0;
     mbar_fence_init();
   }
-  if (tid < 2 * kTreeMaxWords) s_poison[tid] = 0;
+  if (tid < 4 * kTreeMaxWords) s_poison[0][tid] = 0;
   if (warp == kFirstLoad && lane == 0) {
     tma_prefetch_desc(&p.k_map);
     tma_prefetch_desc(&p.v_map);
@@ -198,41 +236,41 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
   // ---- where the sequences lie on the line ---------------------------------------------------------------
   const int n_tab = min(p.B, kSeqTable);
   for (int b = tid; b < p.B; b += kThreads) {
-    const long long n = Walk::span(p, b);
+    const int n = Walk::units(p, b) * Walk::length(p, b);
     if (b < kSeqTable) s_base[b] = n;
-    else if (n) atomicAdd(&s_rest, (unsigned long long)n);
+    else if (n) atomicAdd(&s_rest, n);
   }
   __syncthreads();
-  long long total;
+  int total;
   {
     // every warp scans the table, and warp 0 leaves the result there
     const int run = (n_tab + 31) / 32, lo = min(lane * run, n_tab), hi = min(lo + run, n_tab);
-    long long mine = 0;
+    int mine = 0;
     for (int b = lo; b < hi; ++b) mine += s_base[b];
-    long long end = mine;
+    int end = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long below = __shfl_up_sync(0xffffffffu, end, o);
+      const int below = __shfl_up_sync(0xffffffffu, end, o);
       if (lane >= o) end += below;
     }
     total = __shfl_sync(0xffffffffu, end, 31);
     __syncthreads();
     if (warp == 0) {
-      long long at = end - mine;
+      int at = end - mine;
       for (int b = lo; b < hi; ++b) {
-        const long long n = s_base[b];
+        const int n = s_base[b];
         s_base[b] = at;
         at += n;
       }
     }
     __syncthreads();
   }
-  const long long in_table = total;
-  total += (long long)s_rest;
-  const long long share = max((total + gridDim.x - 1) / (long long)gridDim.x, 1LL);
+  const int in_table = total;
+  total += s_rest;
+  const int share = max((int)(((unsigned)total + gridDim.x - 1) / gridDim.x), 1);
   Walk walk;
-  walk.gcur = (long long)blockIdx.x * share;
-  walk.g1 = min(total, walk.gcur + share);
+  walk.gcur = p.whole ? (int)blockIdx.x : (int)min((long long)blockIdx.x * share, (long long)total);
+  walk.g1 = p.whole ? total : min(total, walk.gcur + share);
   if (walk.gcur < in_table) {
     int lo = 0, hi = n_tab;                        // the last sequence that starts at or before the share
     while (hi - lo > 1) {
@@ -246,14 +284,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     walk.base = in_table;
   }
   __syncthreads();                                 // the table's place is Q's from here on
-  Segment seg;
+  Segment seg{};
   bool ok = true;
   uint32_t gt = 0;                                 // KV tiles this CTA has been through: fixes slots and phases
 
   if (warp < kSmWarps) {
     // =========================== softmax ===========================
-    // 2 * 208 + 88 registers per thread of a warpgroup are what the block was launched with, 3 * 168
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // 2 * 216 + 72 registers per thread of a warpgroup are what the block was launched with, 3 * 168
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int st = warp >> 2;                      // this warpgroup's stream
     const int quad = warp & 3, row = 32 * quad + lane;
     const uint32_t tq = tmem + ((uint32_t)(32 * quad) << 16);
@@ -263,36 +301,28 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     const float2 sl22 = make_float2(sl2, sl2);
     uint32_t steps = 0, n_seg = 0;                 // of this stream, over all segments
 
-    // rows that no unit covers: those of sequences without a token here, and those behind the last sequence
-    {
-      auto clear = [&](int r0, int r1) {
-        for (int64_t i = (int64_t)r0 * p.Hq * 16 + tid; i < (int64_t)r1 * p.Hq * 16; i += 32 * kSmWarps) {
-          reinterpret_cast<uint4*>(p.o)[i] = make_uint4(0, 0, 0, 0);
-          if (i % 16 == 0) p.lse[i / 16] = -INFINITY;
-        }
-      };
-      for (int b = blockIdx.x; b < p.B; b += gridDim.x)
-        if (seq_len_of(p, b) == 0) clear(row0_of(p, b), row0_of(p, b + 1));
-      for (int r = row0_of(p, p.B) + blockIdx.x; r < p.rows; r += gridDim.x) clear(r, r + 1);
-    }
+    // Q of a segment into shared memory: K-major, 128-byte swizzle, halves of 64 dims
+    auto load_q = [&](const Segment& sg, uint32_t n) {
+      const int unit_row = (MT == 2 ? kRows * st : 0) + row, grow = sg.rg * kRows * MT + unit_row, node = grow / group;
+      uint8_t* dst = smem + (MT == 2 ? st : n & 1) * kSlotBytes;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(sg.row0 + node) * p.q_sr + (int64_t)(sg.kvh * group + grow - node * group) * p.q_sh);
+      const bool valid = unit_row < sg.n_rows;
+      const int c0 = MT == 1 ? 8 * st : 0;
+#pragma unroll
+      for (int c = 0; c < (MT == 1 ? 8 : 16); ++c)
+        *reinterpret_cast<uint4*>(dst + ((c0 + c) >> 3) * kHalf + swz128(row, c & 7)) = valid ? __ldg(src + c0 + c) : make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+    };
+    bool more = walk.next(p, seg);
+    if (more) load_q(seg, 0);
 
-    while (ok && walk.next(p, seg)) {
+    while (ok && more) {
       const int unit_row = (MT == 2 ? kRows * st : 0) + row;         // row of the unit
       const bool valid = unit_row < seg.n_rows;
       const int grow = seg.rg * kRows * MT + unit_row, node = grow / group;
       const int64_t qrow = seg.row0 + node, head = seg.kvh * group + grow - node * group;
-      // ---- Q into shared memory: K-major, 128-byte swizzle, halves of 64 dims ---------------------------------
-      {
-        const int c0 = MT == 1 ? 8 * st : 0, cn = MT == 1 ? 8 : 16;
-        uint8_t* dst = smem + (MT == 2 ? st * kSlotBytes : 0);
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + qrow * p.q_sr + head * p.q_sh);
-#pragma unroll
-        for (int c = c0; c < c0 + cn; ++c)
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf + swz128(row, c & 7)) = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full);
-      }
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       const int committed = seg.len - min(max(p.draft_lens[seg.b], 0), seg.len);
       const uint64_t* words = p.mask + (valid ? qrow : 0) * p.mask_stride;
@@ -327,45 +357,54 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
                 }
               if (!bad) continue;
               const int d = tok0 + tok - committed;
-              if (d < 64 * kTreeMaxWords) atomicOr(&s_poison[d >> 5], 1u << (d & 31));
+              if (d < 64 * kTreeMaxWords) atomicOr(&s_poison[n_seg & 1][d >> 5], 1u << (d & 31));
             }
             *at = x;
           }
           fence_proxy_async_smem();
         }
         if (warp_valid) {
-          uint32_t v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
-          tmem_ld_wait();
           if (special) {
-#pragma unroll
+            // masked scores become -inf where they lie; what is rare is kept in short loops, for the sake of the instruction cache
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t seen = mask_bits(words, p.words, tok0 + 32 * c - committed);
               const int left = seg.len - tok0 - 32 * c;
               if (left < 32) seen &= left <= 0 ? 0u : (1u << left) - 1u;
+              uint32_t x[32];
+              tmem_ld_x32(tq + col_s + 32 * c, x);
+              tmem_ld_wait();
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if ((seen >> j & 1u) == 0) v[c][j] = 0xff800000u;                // -inf
+                if ((seen >> j & 1u) == 0) x[j] = 0xff800000u;
+              tmem_st_x32(tq + col_s + 32 * c, x);
             }
+            tmem_st_wait();
           }
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
+          tmem_ld_wait();
           float mx[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
+          for (int c = 0; c < 4; ++c) mx[c] = max_nan(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
 #pragma unroll
           for (int j = 2; j < 32; j += 2)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])));
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2 - kBias;
+            for (int c = 0; c < 4; ++c) mx[c] = max_nan(mx[c], __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
+          // a NaN or +inf among the scores makes the row's maximum NaN, and so all that is computed with it
+          float top = max_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]) * sl2 - kBias;
+          if (top == INFINITY) top = __int_as_float(0x7fffffff);
           float alpha = 1.f;
-          if (top > m + kRescale || m == -INFINITY) {
-            const float m_new = fmaxf(m, top);
+          if (m == -INFINITY || !(top <= m + kRescale)) {
+            const float m_new = max_nan(m, top);
             alpha = m == m_new ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - m_new);
             l *= alpha;
             m = m_new;
           }
           if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
             // the scores' commit covers the P V before them: O is complete
+#pragma unroll 1
             for (int c0 = 0; c0 < kD; c0 += 16) {
               uint32_t x[16];
               tmem_ld_32x32b_x16(tq + col_o + c0, x);
@@ -382,11 +421,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
           float2 f2 = sl22;
           if (__any_sync(0xffffffffu, fabsf(mn) > 16777216.f)) {
             f2 = make_float2(1.f, 1.f);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t x[32];
+              tmem_ld_x32(tq + col_s + 32 * c, x);
+              tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * sl2);
+              tmem_st_x32(tq + col_s + 32 * c, x);
+            }
+            tmem_st_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[c][j] = __float_as_uint(__uint_as_float(v[c][j]) * sl2);
+            for (int c = 0; c < 4; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
+            tmem_ld_wait();
           }
+          // P in two halves, so that P V of the first runs under the exponentials of the second.  The exponentials are what the
+          // softmax warps are bound by (16 a cycle and SM), so some go to the FMA pipe.
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -394,80 +444,117 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float2 d = fma2(make_float2(__uint_as_float(v[c][2 * j]), __uint_as_float(v[c][2 * j + 1])), f2, mn2);
-              const float2 e = make_float2(fast_exp2(d.x), fast_exp2(d.y));
+              const float2 e = (j * kPolyOf8) % 8 < kPolyOf8 ? poly_exp2(d) : make_float2(fast_exp2(d.x), fast_exp2(d.y));
               sum = add2(sum, e);
               pk[j] = pack2<BF16>(e.x, e.y);
             }
             tmem_st_x16(tq + col_s + 16 * c, pk);
+            if (c & 1) {
+              tmem_st_wait();
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[st][c >> 1]);
+            }
           }
           l += sum.x + sum.y;
-          tmem_st_wait();
+        } else if (lane == 0) {
+          mbar_arrive(&p_full[st][0]);
+          mbar_arrive(&p_full[st][1]);
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[st]);
       }
 
-      // ---- O of the segment: join the streams, normalise, write the result or a piece ----------------------
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full, n_seg & 1, deadline));
-      ++n_seg;
-      s_m[st][row] = m;
-      s_l[st][row] = l;
-      bar_sync_named(1, 32 * kSmWarps);
-      tc_fence_after_sync();
+      // ---- the next segment's Q, while this one's last products run: its place is not read any more ------------
+      Segment nx;
+      more = ok && walk.next(p, nx);
+      if (more) load_q(nx, n_seg + 1);
+
+      // ---- join the streams -------------------------------------------------------------------------------------
       const bool both = MT == 1 && seg.count > 1;
-      float f0 = 1.f, f1 = 0.f, M = m, L = l;
+      float f0, f1 = 0.f, M = m, L = l;
       if (MT == 1) {
-        const float m0 = s_m[0][row], m1 = both ? s_m[1][row] : -INFINITY;
-        M = fmaxf(m0, m1);
-        f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - M);
-        f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - M);
-        L = s_l[0][row] * f0 + (both ? s_l[1][row] * f1 : 0.f);
+        if (st == 1) {
+          s_x[0][row] = m;
+          s_x[1][row] = l;
+        }
+        bar_sync_named(1, 32 * kSmWarps);
+        if (st == 0) {
+          const float m1 = both ? s_x[0][row] : -INFINITY;
+          M = max_nan(m, m1);
+          f0 = m == -INFINITY ? 0.f : fast_exp2(m - M);
+          f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - M);
+          L = l * f0 + (both ? s_x[1][row] * f1 : 0.f);
+          const float inv = L == 0.f ? 0.f : 1.f / L;                // a NaN stays one
+          f0 *= inv;
+          f1 *= inv;
+          s_x[0][row] = f0;
+          s_x[1][row] = f1;
+        }
+        bar_sync_named(1, 32 * kSmWarps);
+        if (st == 1) {
+          f0 = s_x[0][row];
+          f1 = s_x[1][row];
+        }
+      } else {
+        f0 = L == 0.f ? 0.f : 1.f / L;
       }
-      const float inv = L == 0.f ? 0.f : 1.f / L;                    // a NaN stays one
-      f0 *= inv;
-      f1 *= inv;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full, n_seg & 1, deadline));
+      tc_fence_after_sync();
+
+      // ---- write the result or a piece ----------------------------------------------------------------------------
+      uint32_t* const poison = s_poison[n_seg & 1];
       uint32_t poisoned = 0;
 #pragma unroll
-      for (int w = 0; w < 2 * kTreeMaxWords; ++w) poisoned |= s_poison[w];
+      for (int w = 0; w < 2 * kTreeMaxWords; ++w) poisoned |= poison[w];
       const bool whole = seg.count == seg.n_tiles;
       // slot 1: the piece that starts its unit; a CTA has at most one of each kind
       const int64_t piece = ((int64_t)blockIdx.x * 2 + (seg.t_begin == 0 ? 1 : 0)) * kRows * MT + unit_row;
       const int c_begin = MT == 1 ? 64 * st : 0, c_end = MT == 1 ? c_begin + 64 : kD;
       if (warp_valid) {
-        for (int c0 = c_begin; c0 < c_end; c0 += 16) {
-          uint32_t x[16], y[16];
-          tmem_ld_32x32b_x16(tq + (MT == 1 ? kColO : col_o) + c0, x);
-          if (both) tmem_ld_32x32b_x16(tq + kColO + 128 + c0, y);
+        uint8_t* out = whole ? reinterpret_cast<uint8_t*>(p.o) + (qrow * p.Hq + head) * (kD * 2) : reinterpret_cast<uint8_t*>(p.part_o + piece * kD);
+#pragma unroll 1
+        for (int c0 = c_begin; c0 < c_end; c0 += 32) {
+          uint32_t x[32], y[32];
+          tmem_ld_x32(tq + (MT == 1 ? kColO : col_o) + c0, x);
+          if (both) tmem_ld_x32(tq + kColO + 128 + c0, y);
           tmem_ld_wait();
-          float o[16];
+          float o[32];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
+          for (int j = 0; j < 32; ++j) {
             o[j] = f0 == 0.f ? 0.f : __uint_as_float(x[j]) * f0;
-            if (both && f1 != 0.f) o[j] += __uint_as_float(y[j]) * f1;
+            if (both) o[j] += f1 == 0.f ? 0.f : __uint_as_float(y[j]) * f1;
           }
-          if (poisoned != 0 && valid) {
-            for (int d = 0; d < 64 * p.words; ++d) {
-              const int tok = committed + d;
-              if ((s_poison[d >> 5] >> (d & 31) & 1u) == 0 || (words[d >> 6] >> (d & 63) & 1u) == 0 || tok >= seg.len) continue;
-              const int pg = p.block_table[seg.b * p.bt_stride + tok / p.page_size];
-              if (pg < 0 || pg >= p.n_pages) continue;
-              const uint16_t* src = p.v + pg * p.v_sp + (tok % p.page_size) * p.v_st + seg.kvh * p.v_sh + c0;
-              for (int j = 0; j < 16; ++j)
-                if (not_finite<BF16>(src[j])) o[j] += widen<BF16>(src[j]);
+          // whole sectors: 16-byte stores, a row per thread, took 13 us per segment of 256 rows
+          if (valid && whole) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = pack2<BF16>(o[2 * j], o[2 * j + 1]);
+            st_global_x8(out + c0 * 2, x);
+            st_global_x8(out + c0 * 2 + 32, x + 8);
+          } else if (valid) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(o[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) st_global_x8(out + c0 * 4 + 32 * j, x + 8 * j);
+          }
+          __syncwarp();
+        }
+        if (poisoned != 0 && valid) {
+          // the elements that were cleared, to the rows that see their token: a finite sum plus an infinity is that infinity
+          for (int d = 0; d < 64 * p.words; ++d) {
+            const int tok = committed + d;
+            if (tok >= seg.len || (poison[d >> 5] >> (d & 31) & 1u) == 0 || (words[d >> 6] >> (d & 63) & 1u) == 0) continue;
+            const int pg = p.block_table[seg.b * p.bt_stride + tok / p.page_size];
+            if (pg < 0 || pg >= p.n_pages) continue;
+            const uint16_t* src = p.v + pg * p.v_sp + (tok % p.page_size) * p.v_st + seg.kvh * p.v_sh;
+#pragma unroll 1
+            for (int c = c_begin; c < c_end; ++c) {
+              if (!not_finite<BF16>(src[c])) continue;
+              if (whole) {
+                uint16_t* e = reinterpret_cast<uint16_t*>(out) + c;
+                *e = (uint16_t)pack2<BF16>(widen<BF16>(*e) + widen<BF16>(src[c]), 0.f);
+              } else {
+                reinterpret_cast<float*>(out)[c] += widen<BF16>(src[c]);
+              }
             }
-          }
-          if (!valid) continue;
-          if (whole) {
-            uint4* dst = reinterpret_cast<uint4*>(p.o + (qrow * p.Hq + head) * kD + c0);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              dst[j] = make_uint4(pack2<BF16>(o[8 * j], o[8 * j + 1]), pack2<BF16>(o[8 * j + 2], o[8 * j + 3]),
-                                  pack2<BF16>(o[8 * j + 4], o[8 * j + 5]), pack2<BF16>(o[8 * j + 6], o[8 * j + 7]));
-          } else {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + piece * kD + c0);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
         }
         if (valid && (MT == 2 || st == 0)) {
@@ -477,13 +564,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
         }
       }
       tc_fence_before_sync();
-      // O, s_m, s_l and s_poison are free; a warp that gave up takes the others with it, or they would wait for it
+      // O and s_x are free; a warp that gave up takes the others with it, or they would wait for it
       if (bar_or_named(1, 32 * kSmWarps, ok ? 0 : 1)) ok = false;
-      if (poisoned != 0 && tid < 2 * kTreeMaxWords) s_poison[tid] = 0;
+      if (tid < 2 * kTreeMaxWords) poison[tid] = 0;                  // used again after the next segment's barrier
+      ++n_seg;
       gt += seg.count;
+      if (more) seg = nx;
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   }
   if (warp >= kFirstLoad) {
     // =========================== loads ===========================
@@ -530,6 +619,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     }
   } else if (warp == kMmaWarp) {
     // =========================== MMA issue ===========================
+    // rows that no unit covers: those of sequences without a token here, and those behind the last sequence
+    {
+      auto clear = [&](int r0, int r1) {
+        for (int64_t i = (int64_t)r0 * p.Hq * 16 + lane; i < (int64_t)r1 * p.Hq * 16; i += 32) {
+          reinterpret_cast<uint4*>(p.o)[i] = make_uint4(0, 0, 0, 0);
+          if (i % 16 == 0) p.lse[i / 16] = -INFINITY;
+        }
+      };
+      for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+        if (seq_len_of(p, b) == 0) clear(row0_of(p, b), row0_of(p, b + 1));
+      for (int r = row0_of(p, p.B) + blockIdx.x; r < p.rows; r += gridDim.x) clear(r, r + 1);
+    }
     constexpr uint32_t fmt = BF16 ? umma_idesc_bf16(kRows, kTile) : umma_idesc_bf16(kRows, kTile) & ~((1u << 7) | (1u << 10));
     constexpr uint32_t id_s = fmt, id_o = fmt | (1u << 16);          // V is MN-major
     // all 512 columns are this CTA's: tensor memory starts at column 0, and no register holds the base
@@ -537,12 +638,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
                    d_v = umma_desc_mn_sw128(smem_u32(ring), kHalf);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0; };
     uint32_t steps[2] = {0, 0}, n_seg = 0;
+    uint32_t q_at = 0;
     auto scores = [&](int s, int i_lane, bool last_user) {           // S of stream s from tile i
       const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0), slot = r % kSlots;
       if (!wait(&kv_full[slot], (r / kSlots) & 1)) return false;
       tc_fence_after_sync();
       if (elect_one()) {
-        const uint32_t kb = slot * kSlotBytes, qb = MT == 2 ? s * kSlotBytes : 0;
+        const uint32_t kb = slot * kSlotBytes, qb = MT == 2 ? s * kSlotBytes : q_at;
 #pragma unroll
         for (int ks = 0; ks < kD / 16; ++ks) {
           const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
@@ -556,23 +658,35 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     };
     auto values = [&](int s, int i_lane, int k_lane, bool last_user) {   // O of stream s += P V of tile i
       const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0) + 1, later = __shfl_sync(0xffffffffu, k_lane, 0), slot = r % kSlots;
-      if (!wait(&p_full[s], steps[s] & 1) || !wait(&kv_full[slot], (r / kSlots) & 1)) return false;
+      // both at once, a lane each: a wait that has nothing to wait for still takes ~200 cycles
+      bool good = true;
+      if (lane == 0) good = mbar_wait(&p_full[s][0], steps[s] & 1, deadline);
+      else if (lane == 1) good = mbar_wait(&kv_full[slot], (r / kSlots) & 1, deadline);
+      if (__all_sync(0xffffffffu, good) == 0) return false;
+      __syncwarp();
+      tc_fence_after_sync();
+      const uint32_t v_lo = (uint32_t)d_v + (slot * kSlotBytes >> 4), v_hi = (uint32_t)(d_v >> 32);
+      if (elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          if (ks == 0) umma_bf16_ts_first(kColO + 128 * s, kColS + 128 * s, v_lo, v_hi, id_o, later);
+          else umma_bf16_ts(kColO + 128 * s, kColS + 128 * s + 8 * ks, v_lo + ks * 128, v_hi, id_o);
+        }
+      }
+      __syncwarp();
+      if (!wait(&p_full[s][1], steps[s] & 1)) return false;
       ++steps[s];
       tc_fence_after_sync();
       if (elect_one()) {
-        const uint32_t vb = slot * kSlotBytes;
 #pragma unroll
-        for (int ks = 0; ks < kTile / 16; ++ks) {
-          const uint32_t lo = (uint32_t)d_v + ((vb + ks * 2048) >> 4);
-          if (ks == 0) umma_bf16_ts_first(kColO + 128 * s, kColS + 128 * s, lo, (uint32_t)(d_v >> 32), id_o, later);
-          else umma_bf16_ts(kColO + 128 * s, kColS + 128 * s + 8 * ks, lo, (uint32_t)(d_v >> 32), id_o);
-        }
+        for (int ks = 4; ks < 8; ++ks) umma_bf16_ts(kColO + 128 * s, kColS + 128 * s + 8 * ks, v_lo + ks * 128, v_hi, id_o);
         if (last_user) umma_commit(&kv_free[slot]);
       }
       __syncwarp();
       return true;
     };
     while (ok && walk.next(p, seg)) {
+      q_at = (__shfl_sync(0xffffffffu, n_seg, 0) & 1) * kSlotBytes;
       ok = wait(&q_full, n_seg & 1);
       ++n_seg;
       if (!ok) break;
@@ -599,11 +713,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
   if (!ok && lane == 0) atomicCAS(p.error_flag, 0, (int)kTimeoutMbarrier);
 
   // ---- what the fold has to do: the unit that this CTA begins and the next ones finish ---------------------
-  if (tid == 0) {
-    Walk w = walk;                                 // at the end of the share: seg is its last segment
+  if (tid == 0 && !p.whole) {
     int4 note = make_int4(-1, 0, 0, 0);
-    if (w.gcur > (long long)blockIdx.x * share && seg.t_begin == 0 && seg.count < seg.n_tiles)
-      note = make_int4(seg.b, seg.kvh, seg.rg, (int)((w.gcur - seg.count + seg.n_tiles - 1) / share));
+    if (seg.count > 0 && seg.t_begin == 0 && seg.count < seg.n_tiles) note = make_int4(seg.b, seg.kvh, seg.rg, (seg.end - 1) / share);
     reinterpret_cast<int4*>(p.part_lse + tree_notes_at(p.ctas, p.tiles))[blockIdx.x] = note;
   }
   tc_fence_before_sync();
@@ -674,13 +786,14 @@ using Fn = void (*)(TreeDecodeParams);
 
 }  // namespace
 
-int tree_pick_tiles(int group, int max_q) { return (long long)group * max_q > kRows ? 2 : 1; }
-
-int tree_pick_ctas(int B, int Hkv, int group, int max_q, int max_seq_len, int sm_count) {
-  const long long per = (long long)kRows * tree_pick_tiles(group, max_q);
-  const long long tiles = (long long)std::max(B, 1) * Hkv * (((long long)group * std::max(max_q, 1) + per - 1) / per) *
-                          std::max((max_seq_len + kTile - 1) / kTile, 1);
-  return (int)std::min<long long>(tiles, sm_count);
+TreePlan tree_plan(int B, int Hkv, int group, int max_q, int max_seq_len, int sm_count) {
+  TreePlan t;
+  t.tiles = (long long)group * max_q > kRows ? 2 : 1;
+  const long long per = (long long)kRows * t.tiles, n_tiles = std::max((max_seq_len + kTile - 1) / kTile, 1);
+  const long long units = (long long)std::max(B, 1) * Hkv * (((long long)group * std::max(max_q, 1) + per - 1) / per);
+  t.whole = units <= sm_count && n_tiles <= kWholeTiles;
+  t.ctas = (int)std::min<long long>(t.whole ? units : units * n_tiles, sm_count);
+  return t;
 }
 
 cudaError_t launch_tree_decode(const TreeDecodeParams& p, bool pdl, cudaStream_t stream) {
@@ -711,9 +824,9 @@ cudaError_t launch_tree_decode(const TreeDecodeParams& p, bool pdl, cudaStream_t
   cfg.attrs = &attr;
   cfg.numAttrs = pdl ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, fn, p);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || p.whole) return e;
   // the fold is always chained to this launch; it waits for the whole grid before it reads a piece
-  cfg.gridDim = dim3(p.ctas, 8, 1);
+  cfg.gridDim = dim3(p.ctas, 16, 1);
   cfg.blockDim = dim3(kFoldThreads, 1, 1);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;

@@ -27,6 +27,7 @@ struct TreeDecodeParams {
   int* error_flag;
   int rows, B, Hq, Hkv, page_size, max_pages, n_pages, box_tok, words;
   int ctas, tiles;                 // tiles of 128 rows that a CTA works on: 1 or 2
+  int whole;                       // 1: CTAs take units from end to end, nothing is split and no second kernel runs
   int is_bf16, lse_base2;
   float scale;
   unsigned long long timeout_ns;
@@ -36,9 +37,15 @@ constexpr int kTreeMaxWords = 4;
 constexpr size_t tree_part_o_floats(int ctas, int tiles) { return (size_t)2 * ctas * 128 * tiles * 128; }
 constexpr size_t tree_notes_at(int ctas, int tiles) { return (size_t)2 * ctas * 128 * tiles; }     // in part_lse
 constexpr size_t tree_part_lse_floats(int ctas, int tiles) { return tree_notes_at(ctas, tiles) + (size_t)ctas * 4; }
-// row tiles per CTA, and CTAs, for up to max_q new tokens per sequence and max_seq_len tokens of the longest
-int tree_pick_tiles(int group, int max_q);
-int tree_pick_ctas(int B, int Hkv, int group, int max_q, int max_seq_len, int sm_count);
+// how a call with up to max_q new tokens per sequence and max_seq_len tokens of the longest is divided
+struct TreePlan {
+  int tiles, ctas, whole;
+};
+TreePlan tree_plan(int B, int Hkv, int group, int max_q, int max_seq_len, int sm_count);
+// places on the line that the KV tiles lie on (see tree_attn.cu), at most: counted in 32 bits
+constexpr int64_t tree_line_bound(int64_t rows, int64_t B, int64_t Hkv, int64_t group, int64_t max_tokens) {
+  return (rows * group / 128 + B) * Hkv * (max_tokens / 128 + 4);
+}
 
 cudaError_t launch_tree_decode(const TreeDecodeParams& p, bool pdl, cudaStream_t stream);
 
