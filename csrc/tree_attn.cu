@@ -24,6 +24,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "helix_common.cuh"
 #include "sm100.cuh"
@@ -36,14 +37,13 @@ using namespace sm100;
 constexpr int kD = 128, kTile = 128, kRows = 128;
 constexpr int kSlotBytes = kTile * kD * 2;             // 32768: one K or V tile, two halves of [128 tokens x 64 dims]
 constexpr int kHalf = kTile * 128;                     // 16384
-constexpr int kSmWarps = 8, kMmaWarp = 8, kFirstLoad = 9, kLoadWarps = 3, kThreads = 384;
+constexpr int kSmWarps = 8, kMmaWarp = 8, kFirstLoad = 10, kLoadWarps = 2, kThreads = 384;      // an MMA warp per stream
 constexpr int kSlots = 5;                              // beside two tiles of Q
 constexpr int kSmem = (2 + kSlots) * kSlotBytes + 1024;
 constexpr uint32_t kColS = 0, kColO = 256;             // S0, S1, O0, O1: 128 columns each; P lies over its S
 constexpr int kSeqTable = 512;
 constexpr int kWholeTiles = 4;                         // units of up to so many tiles stay whole, a CTA each
 constexpr int kUnitCost = 2;                           // what a unit costs besides its tiles, in tiles
-constexpr int kPolyOf8 = 3;                            // of 8 pairs of exponentials, how many the FMA pipe computes
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;                        // the running maximum moves when a row's grew by more than 2^8
 
@@ -58,21 +58,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=l"(r)
       : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
   return *reinterpret_cast<float2*>(&r);
-}
-// 2^x for two numbers up to 127, on the FMA pipe: 2^n times a polynomial in f = x - n, |f| <= 1/2, which is 2^f to 1.5e-5 (equal
-// error at all extrema, 1 at f = 0), far below the step of bf16 and fp16 that P is rounded to.  Below 2^-126 comes exactly 0.
-__device__ __forceinline__ float2 poly_exp2(float2 x) {
-  const float2 magic = make_float2(12582912.f, 12582912.f), neg = make_float2(-12582912.f, -12582912.f);     // 1.5 * 2^23
-  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const float2 t = add2(x, magic), n = add2(t, neg), f = fma2(n, make_float2(-1.f, -1.f), x);
-  float2 r = make_float2(0x1.564e84p-7f, 0x1.564e84p-7f);
-  r = fma2(r, f, make_float2(0x1.cc088cp-5f, 0x1.cc088cp-5f));
-  r = fma2(r, f, make_float2(0x1.eba26ap-3f, 0x1.eba26ap-3f));
-  r = fma2(r, f, make_float2(0x1.62da5ap-1f, 0x1.62da5ap-1f));
-  r = fma2(r, f, make_float2(1.f, 1.f));
-  r = make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
-                  __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
-  return add2(r, make_float2(-0x1p-126f, -0x1p-126f));
 }
 // maxima that pass a NaN on
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -189,7 +174,7 @@ __device__ __forceinline__ uint32_t mask_bits(const uint64_t* words, int n_words
 template <bool BF16, int MT>
 __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_constant__ TreeDecodeParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t kv_full[kSlots], kv_free[kSlots], s_full[2], p_full[2][2], o_full, q_full, drain;
+  __shared__ __align__(8) uint64_t kv_full[kSlots], kv_free[kSlots], s_full[2], p_full[2][2], o_full, q_full, scrubbed, turn[2], drain[2];
   __shared__ uint32_t tmem_slot, s_poison[2][2 * kTreeMaxWords];      // by turns: a segment's is cleared behind its end
   __shared__ float s_x[2][kRows];                  // what the streams tell each other at the end of a segment
   __shared__ int s_rest;
@@ -203,16 +188,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
   if (tid == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&kv_full[i], kLoadWarps);          // each announces its own bytes
-      mbar_init(&kv_free[i], 1);
+      mbar_init(&kv_free[i], MT);                  // every stream that reads the tile
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i][0], 4);                 // halves of 64 tokens
       mbar_init(&p_full[i][1], 4);
+      mbar_init(&turn[i], 4);
     }
-    mbar_init(&o_full, 1);
+    mbar_init(&o_full, 2);
     mbar_init(&q_full, kSmWarps);
-    mbar_init(&drain, 1);
+    mbar_init(&scrubbed, kSmWarps);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     s_rest = 0;
     mbar_fence_init();
   }
@@ -299,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     constexpr float kBias = BF16 ? 0.f : 7.f;
     const float sl2 = p.scale * kLog2e;
     const float2 sl22 = make_float2(sl2, sl2);
-    uint32_t steps = 0, n_seg = 0;                 // of this stream, over all segments
+    uint32_t steps = 0, n_seg = 0, n_scrub = 0;    // of this stream, over all segments
 
     // Q of a segment into shared memory: K-major, 128-byte swizzle, halves of 64 dims
     auto load_q = [&](const Segment& sg, uint32_t n) {
@@ -336,13 +324,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[st], steps & 1, deadline));
         if (!ok) break;
         tc_fence_after_sync();
-        if (special && (MT == 1 || st == 0)) {
-          // V: rows behind the sequence become zeros, elements of drafted tokens that are not finite too
+        if (special) {
+          // V: rows behind the sequence become zeros, elements of drafted tokens that are not finite too.  A tile that both streams read
+          // is shared out, and neither stream's P V starts before it is done.
           const uint32_t r = 2 * (gt + i) + 1;
           uint8_t* v = ring + (r % kSlots) * kSlotBytes;
           ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[r % kSlots], (r / kSlots) & 1, deadline));
           if (!ok) break;
-          for (int tok = max(committed - tok0, 0) + (row >> 4); tok < kTile; tok += 8) {
+          const int who = MT == 2 ? tid : row;
+          for (int tok = max(committed - tok0, 0) + (who >> 4); tok < kTile; tok += 8 * MT) {
             uint4* at = reinterpret_cast<uint4*>(v + ((row >> 3) & 1) * kHalf + swz128(tok, row & 7));
             uint4 x = make_uint4(0, 0, 0, 0);
             if (tok0 + tok < seg.len) {
@@ -362,6 +352,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             *at = x;
           }
           fence_proxy_async_smem();
+          if (MT == 2) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&scrubbed);
+            ok = __all_sync(0xffffffffu, mbar_wait(&scrubbed, n_scrub & 1, deadline));
+            ++n_scrub;
+            if (!ok) break;
+          }
         }
         if (warp_valid) {
           if (special) {
@@ -435,8 +432,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             for (int c = 0; c < 4; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
             tmem_ld_wait();
           }
-          // P in two halves, so that P V of the first runs under the exponentials of the second.  The exponentials are what the
-          // softmax warps are bound by (16 a cycle and SM), so some go to the FMA pipe.
+          // The exponentials are what a step is made of (16 a cycle and SM: 1024 cycles a tile).  Two streams that start on the same KV tile
+          // would stay in step, both at their exponentials and then both waiting for the tensor cores, so they take turns.
+          if (MT == 2) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&turn[st], (steps & 1) ^ (st == 0 ? 1 : 0), deadline));
+            if (!ok) break;
+          }
+          // P in two halves, so that P V of the first runs under the exponentials of the second
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -444,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float2 d = fma2(make_float2(__uint_as_float(v[c][2 * j]), __uint_as_float(v[c][2 * j + 1])), f2, mn2);
-              const float2 e = (j * kPolyOf8) % 8 < kPolyOf8 ? poly_exp2(d) : make_float2(fast_exp2(d.x), fast_exp2(d.y));
+              const float2 e = make_float2(fast_exp2(d.x), fast_exp2(d.y));
               sum = add2(sum, e);
               pk[j] = pack2<BF16>(e.x, e.y);
             }
@@ -457,10 +459,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             }
           }
           l += sum.x + sum.y;
-        } else if (lane == 0) {
-          mbar_arrive(&p_full[st][0]);
-          mbar_arrive(&p_full[st][1]);
+        } else {
+          if (MT == 2) ok = __all_sync(0xffffffffu, mbar_wait(&turn[st], (steps & 1) ^ (st == 0 ? 1 : 0), deadline));
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive(&p_full[st][0]);
+            mbar_arrive(&p_full[st][1]);
+          }
         }
+        if (MT == 2 && lane == 0) mbar_arrive(&turn[st ^ 1]);
       }
 
       // ---- the next segment's Q, while this one's last products run: its place is not read any more ------------
@@ -617,10 +624,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       const unsigned long long limit = now_ns() + 10000000ull;
       for (uint32_t r = issued > (uint32_t)kSlots ? issued - kSlots : 0; r < issued; ++r) mbar_wait(&kv_full[r % kSlots], (r / kSlots) & 1, limit);
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp >= kMmaWarp) {
     // =========================== MMA issue ===========================
+    // A warp per stream: one warp for both, in a fixed order, held a stream up behind the other (128k tokens, 64 drafted 315 us).
     // rows that no unit covers: those of sequences without a token here, and those behind the last sequence
-    {
+    if (warp == kMmaWarp) {
       auto clear = [&](int r0, int r1) {
         for (int64_t i = (int64_t)r0 * p.Hq * 16 + lane; i < (int64_t)r1 * p.Hq * 16; i += 32) {
           reinterpret_cast<uint4*>(p.o)[i] = make_uint4(0, 0, 0, 0);
@@ -637,78 +645,78 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     const uint64_t d_q = umma_desc_k_sw128(smem_u32(smem)), d_k = umma_desc_k_sw128(smem_u32(ring)),
                    d_v = umma_desc_mn_sw128(smem_u32(ring), kHalf);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0; };
-    uint32_t steps[2] = {0, 0}, n_seg = 0;
-    uint32_t q_at = 0;
-    auto scores = [&](int s, int i_lane, bool last_user) {           // S of stream s from tile i
+    // (the stream is a constant of the code, so that the columns are: an operand that is not known to be the same in all lanes costs
+    // an MMA some 100 cycles)
+    auto role = [&](auto stream) {
+    constexpr int st = decltype(stream)::value;
+    constexpr uint32_t col_s = kColS + 128 * st, col_o = kColO + 128 * st;
+    uint32_t steps = 0, n_seg = 0, q_at = 0;
+    auto scores = [&](int i_lane) {                // S of tile i
       const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0), slot = r % kSlots;
       if (!wait(&kv_full[slot], (r / kSlots) & 1)) return false;
       tc_fence_after_sync();
+      const uint32_t kb = slot * kSlotBytes, qb = q_at;
       if (elect_one()) {
-        const uint32_t kb = slot * kSlotBytes, qb = MT == 2 ? s * kSlotBytes : q_at;
 #pragma unroll
         for (int ks = 0; ks < kD / 16; ++ks) {
           const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
-          umma_bf16(kColS + 128 * s, d_q + ((qb + off) >> 4), d_k + ((kb + off) >> 4), id_s, ks > 0);
+          umma_bf16(col_s, d_q + ((qb + off) >> 4), d_k + ((kb + off) >> 4), id_s, ks > 0);
         }
-        umma_commit(&s_full[s]);
-        if (last_user) umma_commit(&kv_free[slot]);
+        umma_commit(&s_full[st]);
+        umma_commit(&kv_free[slot]);
       }
       __syncwarp();
       return true;
     };
-    auto values = [&](int s, int i_lane, int k_lane, bool last_user) {   // O of stream s += P V of tile i
+    auto values = [&](int i_lane, int k_lane) {    // O += P V of tile i
       const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0) + 1, later = __shfl_sync(0xffffffffu, k_lane, 0), slot = r % kSlots;
-      // both at once, a lane each: a wait that has nothing to wait for still takes ~200 cycles
-      bool good = true;
-      if (lane == 0) good = mbar_wait(&p_full[s][0], steps[s] & 1, deadline);
-      else if (lane == 1) good = mbar_wait(&kv_full[slot], (r / kSlots) & 1, deadline);
-      if (__all_sync(0xffffffffu, good) == 0) return false;
-      __syncwarp();
+      // V first: what is there already still takes a wait's time, which is better spent before P is there
+      if (!wait(&kv_full[slot], (r / kSlots) & 1) || !wait(&p_full[st][0], steps & 1)) return false;
       tc_fence_after_sync();
       const uint32_t v_lo = (uint32_t)d_v + (slot * kSlotBytes >> 4), v_hi = (uint32_t)(d_v >> 32);
       if (elect_one()) {
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          if (ks == 0) umma_bf16_ts_first(kColO + 128 * s, kColS + 128 * s, v_lo, v_hi, id_o, later);
-          else umma_bf16_ts(kColO + 128 * s, kColS + 128 * s + 8 * ks, v_lo + ks * 128, v_hi, id_o);
+          if (ks == 0) umma_bf16_ts_first(col_o, col_s, v_lo, v_hi, id_o, later);
+          else umma_bf16_ts(col_o, col_s + 8 * ks, v_lo + ks * 128, v_hi, id_o);
         }
       }
       __syncwarp();
-      if (!wait(&p_full[s][1], steps[s] & 1)) return false;
-      ++steps[s];
+      if (!wait(&p_full[st][1], steps & 1)) return false;
+      ++steps;
       tc_fence_after_sync();
       if (elect_one()) {
 #pragma unroll
-        for (int ks = 4; ks < 8; ++ks) umma_bf16_ts(kColO + 128 * s, kColS + 128 * s + 8 * ks, v_lo + ks * 128, v_hi, id_o);
-        if (last_user) umma_commit(&kv_free[slot]);
+        for (int ks = 4; ks < 8; ++ks) umma_bf16_ts(col_o, col_s + 8 * ks, v_lo + ks * 128, v_hi, id_o);
+        umma_commit(&kv_free[slot]);
       }
       __syncwarp();
       return true;
     };
     while (ok && walk.next(p, seg)) {
-      q_at = (__shfl_sync(0xffffffffu, n_seg, 0) & 1) * kSlotBytes;
+      q_at = (__shfl_sync(0xffffffffu, MT == 2 ? (uint32_t)st : n_seg, 0) & 1) * kSlotBytes;
       ok = wait(&q_full, n_seg & 1);
       ++n_seg;
       if (!ok) break;
       tc_fence_after_sync();
-      const int n0 = MT == 2 ? seg.count : (seg.count + 1) / 2, n1 = MT == 2 ? seg.count : seg.count / 2;
-      auto tile = [&](int s, int k) { return MT == 2 ? k : 2 * k + s; };
-      ok = scores(0, tile(0, 0), MT == 1);
-      if (ok && n1 > 0) ok = scores(1, tile(1, 0), true);
-      for (int k = 0; k < n0 && ok; ++k) {
-        ok = values(0, tile(0, k), k, MT == 1);
-        if (ok && k + 1 < n0) ok = scores(0, tile(0, k + 1), MT == 1);
-        if (ok && k < n1) ok = values(1, tile(1, k), k, true);
-        if (ok && k + 1 < n1) ok = scores(1, tile(1, k + 1), true);
+      const int n = MT == 2 ? seg.count : (seg.count - st + 1) / 2;
+      auto tile = [&](int k) { return MT == 2 ? k : 2 * k + st; };
+      if (n > 0) ok = scores(tile(0));
+      for (int k = 0; k < n && ok; ++k) {
+        ok = values(tile(k), k);
+        if (ok && k + 1 < n) ok = scores(tile(k + 1));
       }
       if (ok && elect_one()) umma_commit(&o_full);
       __syncwarp();
       gt += seg.count;
     }
     if (!ok) {
-      if (elect_one()) umma_commit(&drain);        // nothing of this CTA's may be in flight when it leaves
-      mbar_wait(&drain, 0, now_ns() + 10000000ull);
+      if (elect_one()) umma_commit(&drain[st]);    // nothing of this CTA's may be in flight when it leaves
+      mbar_wait(&drain[st], 0, now_ns() + 10000000ull);
     }
+    };
+    if (warp == kMmaWarp) role(std::integral_constant<int, 0>{});
+    else role(std::integral_constant<int, 1>{});
   }
   if (!ok && lane == 0) atomicCAS(p.error_flag, 0, (int)kTimeoutMbarrier);
 
