@@ -174,10 +174,11 @@ __device__ __forceinline__ uint32_t mask_bits(const uint64_t* words, int n_words
 template <bool BF16, int MT>
 __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_constant__ TreeDecodeParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t kv_full[kSlots], kv_free[kSlots], s_full[2], p_full[2][2], o_full, q_full, scrubbed, turn[2], drain[2];
+  __shared__ __align__(8) uint64_t kv_full[kSlots], kv_free[kSlots], s_full[2], p_full[2][2], o_full[2], q_full, idle, scrubbed, turn[2], drain[2];
   __shared__ uint32_t tmem_slot, s_poison[2][2 * kTreeMaxWords];      // by turns: a segment's is cleared behind its end
   __shared__ float s_x[2][kRows];                  // what the streams tell each other at the end of a segment
   __shared__ int s_rest;
+  __shared__ uint32_t s_issued;                    // tiles (K and V apart) whose loads have been started
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + 2 * kSlotBytes;           // behind two tiles of Q: both row tiles, or this segment's and the next one's
@@ -195,13 +196,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       mbar_init(&p_full[i][0], 4);                 // halves of 64 tokens
       mbar_init(&p_full[i][1], 4);
       mbar_init(&turn[i], 4);
+      mbar_init(&o_full[i], 1);
     }
-    mbar_init(&o_full, 2);
     mbar_init(&q_full, kSmWarps);
+    mbar_init(&idle, 1);
     mbar_init(&scrubbed, kSmWarps);
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     s_rest = 0;
+    s_issued = 0;
     mbar_fence_init();
   }
   if (tid < 4 * kTreeMaxWords) s_poison[0][tid] = 0;
@@ -276,6 +279,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
   bool ok = true;
   uint32_t gt = 0;                                 // KV tiles this CTA has been through: fixes slots and phases
 
+  // The wait for entry r of the ring.  Loads complete in any order, and with one row tile a stream only sees every other tile: entry
+  // r - kSlots may have been the other stream's and still be on its way, and then the parity of r would be taken for the one before.  The
+  // loader starts an entry when its place has been read to the end, so from then on the parity means r.
+  auto tile_there = [&](uint32_t r) {
+    if (MT == 1) {
+      unsigned spins = 0;
+      while (*reinterpret_cast<volatile uint32_t*>(&s_issued) <= r)
+        if ((++spins & 255u) == 0u && now_ns() > deadline) return false;
+    }
+    return mbar_wait(&kv_full[r % kSlots], (r / kSlots) & 1, deadline);
+  };
+
   if (warp < kSmWarps) {
     // =========================== softmax ===========================
     // 2 * 216 + 72 registers per thread of a warpgroup are what the block was launched with, 3 * 168
@@ -288,6 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     const float sl2 = p.scale * kLog2e;
     const float2 sl22 = make_float2(sl2, sl2);
     uint32_t steps = 0, n_seg = 0, n_scrub = 0;    // of this stream, over all segments
+    uint32_t n_joined = 0, n_idle = 0;             // one row tile: segments in which both streams had a part, and the others
 
     // Q of a segment into shared memory: K-major, 128-byte swizzle, halves of 64 dims
     auto load_q = [&](const Segment& sg, uint32_t n) {
@@ -315,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       const int committed = seg.len - min(max(p.draft_lens[seg.b], 0), seg.len);
       const uint64_t* words = p.mask + (valid ? qrow : 0) * p.mask_stride;
       float m = -INFINITY, l = 0.f;
+      bool huge = false;
       const int n_steps = MT == 2 ? seg.count : (seg.count - st + 1) / 2;
 
       for (int k = 0; k < n_steps; ++k, ++steps) {
@@ -329,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
           // is shared out, and neither stream's P V starts before it is done.
           const uint32_t r = 2 * (gt + i) + 1;
           uint8_t* v = ring + (r % kSlots) * kSlotBytes;
-          ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[r % kSlots], (r / kSlots) & 1, deadline));
+          ok = __all_sync(0xffffffffu, tile_there(r));
           if (!ok) break;
           const int who = MT == 2 ? tid : row;
           for (int tok = max(committed - tok0, 0) + (who >> 4); tok < kTile; tok += 8 * MT) {
@@ -352,8 +369,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             *at = x;
           }
           fence_proxy_async_smem();
+          __syncwarp();
           if (MT == 2) {
-            __syncwarp();
             if (lane == 0) mbar_arrive(&scrubbed);
             ok = __all_sync(0xffffffffu, mbar_wait(&scrubbed, n_scrub & 1, deadline));
             ++n_scrub;
@@ -382,67 +399,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
           tmem_ld_wait();
-          float mx[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = max_nan(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
-#pragma unroll
-          for (int j = 2; j < 32; j += 2)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = max_nan(mx[c], __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
-          // a NaN or +inf among the scores makes the row's maximum NaN, and so all that is computed with it
-          float top = max_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]) * sl2 - kBias;
-          if (top == INFINITY) top = __int_as_float(0x7fffffff);
-          float alpha = 1.f;
-          if (m == -INFINITY || !(top <= m + kRescale)) {
-            const float m_new = max_nan(m, top);
-            alpha = m == m_new ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - m_new);
-            l *= alpha;
-            m = m_new;
-          }
-          if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            // the scores' commit covers the P V before them: O is complete
-#pragma unroll 1
-            for (int c0 = 0; c0 < kD; c0 += 16) {
-              uint32_t x[16];
-              tmem_ld_32x32b_x16(tq + col_o + c0, x);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
-              tmem_st_x16(tq + col_o + c0, x);
-            }
-          }
-          const float mn = m == -INFINITY ? 0.f : -m;
-          const float2 mn2 = make_float2(mn, mn);
-          // m is a rounded product, so s * sl2 - m is off by the rounding, alike for the whole row: up to 2^24 a factor of two at most.
-          // Beyond, the products are rounded too, or the factor could overflow.
-          float2 f2 = sl22;
-          if (__any_sync(0xffffffffu, fabsf(mn) > 16777216.f)) {
-            f2 = make_float2(1.f, 1.f);
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t x[32];
-              tmem_ld_x32(tq + col_s + 32 * c, x);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * sl2);
-              tmem_st_x32(tq + col_s + 32 * c, x);
-            }
-            tmem_st_wait();
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
-            tmem_ld_wait();
-          }
           // The exponentials are what a step is made of (16 a cycle and SM: 1024 cycles a tile).  Two streams that start on the same KV tile
           // would stay in step, both at their exponentials and then both waiting for the tensor cores, so they take turns.
           if (MT == 2) {
             ok = __all_sync(0xffffffffu, mbar_wait(&turn[st], (steps & 1) ^ (st == 0 ? 1 : 0), deadline));
             if (!ok) break;
           }
-          // P in two halves, so that P V of the first runs under the exponentials of the second
-          float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
+          // P in two halves, so that P V of the first runs under the exponentials of the second.  The first half is computed with the
+          // maximum so far, and the tile's own maximum beside it on a pipe that is idle then; if a row's grew by more than 2^8 the
+          // maximum moves and the half is done again.
+          float2 sum;
+          float2 f2 = sl22;
+          uint32_t pk[16];
+          auto half_chunk = [&](int c, float2 mn2) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float2 d = fma2(make_float2(__uint_as_float(v[c][2 * j]), __uint_as_float(v[c][2 * j + 1])), f2, mn2);
@@ -451,13 +420,67 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
               pk[j] = pack2<BF16>(e.x, e.y);
             }
             tmem_st_x16(tq + col_s + 16 * c, pk);
-            if (c & 1) {
-              tmem_st_wait();
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_full[st][c >> 1]);
+          };
+          float mn = m == -INFINITY ? 0.f : -m;
+          for (bool again = false;; again = true) {
+            const float2 mn2 = make_float2(mn, mn);
+            sum = make_float2(0.f, 0.f);
+            if (huge && f2.x != 1.f) {
+              f2 = make_float2(1.f, 1.f);
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[c][j] = __float_as_uint(__uint_as_float(v[c][j]) * sl2);
             }
+            half_chunk(0, mn2);
+            half_chunk(1, mn2);
+            if (again) break;
+            float mx[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mx[c] = max_nan(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
+#pragma unroll
+            for (int j = 2; j < 32; j += 2)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) mx[c] = max_nan(mx[c], __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
+            // a NaN or +inf among the scores makes the row's maximum NaN, and so all that is computed with it
+            float top = max_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]) * f2.x - kBias;
+            if (top == INFINITY) top = __int_as_float(0x7fffffff);
+            // (a row whose maximum is -inf, the first tile's, has nothing to take back if all its scores are -inf)
+            const bool move = !(top <= m + kRescale) && top != -INFINITY;
+            if (!__any_sync(0xffffffffu, move)) break;
+            const float m_new = move ? max_nan(m, top) : m;
+            const float alpha = m == m_new ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - m_new);
+            l *= alpha;
+            m = m_new;
+            tmem_st_wait();                        // the half that will be done again
+            if (k > 0) {
+              // the scores' commit covers the P V before them: O is complete
+#pragma unroll 1
+              for (int c0 = 0; c0 < kD; c0 += 16) {
+                uint32_t x[16];
+                tmem_ld_32x32b_x16(tq + col_o + c0, x);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
+                tmem_st_x16(tq + col_o + c0, x);
+              }
+            }
+            mn = m == -INFINITY ? 0.f : -m;
+            // m is a rounded product, so s * sl2 - m is off by the rounding, alike for the whole row: up to 2^24 a factor of two at most.
+            // Beyond, the products are rounded too, or the factor could overflow.
+            huge |= __any_sync(0xffffffffu, fabsf(mn) > 16777216.f) != 0;
           }
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[st][0]);
+          if (MT == 2 && lane == 0) mbar_arrive(&turn[st ^ 1]);
+          half_chunk(2, make_float2(mn, mn));
+          half_chunk(3, make_float2(mn, mn));
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[st][1]);
           l += sum.x + sum.y;
         } else {
           if (MT == 2) ok = __all_sync(0xffffffffu, mbar_wait(&turn[st], (steps & 1) ^ (st == 0 ? 1 : 0), deadline));
@@ -465,12 +488,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
           if (lane == 0) {
             mbar_arrive(&p_full[st][0]);
             mbar_arrive(&p_full[st][1]);
+            if (MT == 2) mbar_arrive(&turn[st ^ 1]);
           }
         }
-        if (MT == 2 && lane == 0) mbar_arrive(&turn[st ^ 1]);
       }
 
       // ---- the next segment's Q, while this one's last products run: its place is not read any more ------------
+      // (a stream without steps has not heard of its MMA warp: neither may be a phase of q_full ahead of the other)
+      if (n_steps == 0) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&idle, n_idle & 1, deadline));
+        ++n_idle;
+      }
       Segment nx;
       more = ok && walk.next(p, nx);
       if (more) load_q(nx, n_seg + 1);
@@ -504,7 +532,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       } else {
         f0 = L == 0.f ? 0.f : 1.f / L;
       }
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full, n_seg & 1, deadline));
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[MT == 2 ? st : 0], n_seg & 1, deadline));
+      if (ok && both) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[1], n_joined & 1, deadline));
+      n_joined += both;
       tc_fence_after_sync();
 
       // ---- write the result or a piece ----------------------------------------------------------------------------
@@ -571,6 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
         }
       }
       tc_fence_before_sync();
+      __syncwarp();
       // O and s_x are free; a warp that gave up takes the others with it, or they would wait for it
       if (bar_or_named(1, 32 * kSmWarps, ok ? 0 : 1)) ok = false;
       if (tid < 2 * kTreeMaxWords) poison[tid] = 0;                  // used again after the next segment's barrier
@@ -583,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
   }
   if (warp >= kFirstLoad) {
     // =========================== loads ===========================
-    // Boxes of 16 tokens x 64 dims (a page of 16 tokens allows no larger ones): 32 per tile, shared by three warps, each issued by
+    // Boxes of 16 tokens x 64 dims (a page of 16 tokens allows no larger ones): 32 per tile, shared by two warps, each issued by
     // one elected lane of a warp that has stayed together.  One warp whose lanes issued a box each took ~136 cycles per box,
     // 4400 per tile, which bounded everything (64 x 8192 tokens 528 us).
     const int per_tile = kTile / p.box_tok, lw = warp - kFirstLoad;
@@ -604,7 +635,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
           const uint32_t r = 2 * (gt + i) + kv, slot = r % kSlots;
           if (r >= (uint32_t)kSlots) ok = __all_sync(0xffffffffu, mbar_wait(&kv_free[slot], (r / kSlots - 1) & 1, deadline));
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(&kv_full[slot], (uint32_t)mine * p.box_tok * kD);
+          if (lane == 0) {
+            if (lw == 0) *reinterpret_cast<volatile uint32_t*>(&s_issued) = r + 1;
+            mbar_expect_tx(&kv_full[slot], (uint32_t)mine * p.box_tok * kD);
+          }
           __syncwarp();
           for (int j = lw; j < boxes; j += kLoadWarps) {
             const int pg = __shfl_sync(0xffffffffu, page, j >> 1), at = __shfl_sync(0xffffffffu, in_page, j >> 1), half = j & 1;
@@ -619,6 +653,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       }
       gt += seg.count;
     }
+    // the last commits on kv_free have to arrive before this CTA leaves too
+    for (uint32_t r = issued > (uint32_t)kSlots ? issued - kSlots : 0; r < issued && ok; ++r)
+      ok = __all_sync(0xffffffffu, mbar_wait(&kv_free[r % kSlots], (r / kSlots) & 1, deadline));
     if (!ok) {
       // nothing may land in this CTA's shared memory after it has left
       const unsigned long long limit = now_ns() + 10000000ull;
@@ -651,9 +688,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     constexpr int st = decltype(stream)::value;
     constexpr uint32_t col_s = kColS + 128 * st, col_o = kColO + 128 * st;
     uint32_t steps = 0, n_seg = 0, q_at = 0;
-    auto scores = [&](int i_lane) {                // S of tile i
+    auto k_there = [&](int i_lane) {
+      const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0);
+      return __all_sync(0xffffffffu, tile_there(r)) != 0;
+    };
+    auto scores = [&](int i_lane) {                // S of tile i, which is there
       const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0), slot = r % kSlots;
-      if (!wait(&kv_full[slot], (r / kSlots) & 1)) return false;
       tc_fence_after_sync();
       const uint32_t kb = slot * kSlotBytes, qb = q_at;
       if (elect_one()) {
@@ -668,10 +708,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       __syncwarp();
       return true;
     };
-    auto values = [&](int i_lane, int k_lane) {    // O += P V of tile i
+    auto values = [&](int i_lane, int k_lane, int next) {  // O += P V of tile i
       const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0) + 1, later = __shfl_sync(0xffffffffu, k_lane, 0), slot = r % kSlots;
       // V first: what is there already still takes a wait's time, which is better spent before P is there
-      if (!wait(&kv_full[slot], (r / kSlots) & 1) || !wait(&p_full[st][0], steps & 1)) return false;
+      if (__all_sync(0xffffffffu, tile_there(r)) == 0 || !wait(&p_full[st][0], steps & 1)) return false;
       tc_fence_after_sync();
       const uint32_t v_lo = (uint32_t)d_v + (slot * kSlotBytes >> 4), v_hi = (uint32_t)(d_v >> 32);
       if (elect_one()) {
@@ -682,7 +722,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
         }
       }
       __syncwarp();
-      if (!wait(&p_full[st][1], steps & 1)) return false;
+      // two row tiles: the next K is there by now, and is looked for while P is not.  One: the cache may be what everything waits for,
+      // and this V's place is needed
+      if ((MT == 2 && next >= 0 && !k_there(next)) || !wait(&p_full[st][1], steps & 1)) return false;
       ++steps;
       tc_fence_after_sync();
       if (elect_one()) {
@@ -695,18 +737,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     };
     while (ok && walk.next(p, seg)) {
       q_at = (__shfl_sync(0xffffffffu, MT == 2 ? (uint32_t)st : n_seg, 0) & 1) * kSlotBytes;
+      const int n = MT == 2 ? seg.count : (seg.count - st + 1) / 2;
       ok = wait(&q_full, n_seg & 1);
       ++n_seg;
       if (!ok) break;
       tc_fence_after_sync();
-      const int n = MT == 2 ? seg.count : (seg.count - st + 1) / 2;
       auto tile = [&](int k) { return MT == 2 ? k : 2 * k + st; };
-      if (n > 0) ok = scores(tile(0));
+      if (n > 0) ok = k_there(tile(0)) && scores(tile(0));
       for (int k = 0; k < n && ok; ++k) {
-        ok = values(tile(k), k);
-        if (ok && k + 1 < n) ok = scores(tile(k + 1));
+        ok = values(tile(k), k, k + 1 < n ? tile(k + 1) : -1);
+        if (ok && k + 1 < n) ok = (MT == 2 || k_there(tile(k + 1))) && scores(tile(k + 1));
       }
-      if (ok && elect_one()) umma_commit(&o_full);
+      if (ok && elect_one()) {
+        if (n > 0) umma_commit(&o_full[st]);
+        else mbar_arrive(&idle);
+      }
       __syncwarp();
       gt += seg.count;
     }

@@ -206,6 +206,17 @@ def test_many_sequences():
     check(s, "HND", "bf16", max_seq_len=90, max_q_len=3)
 
 
+@pytest.mark.parametrize("t,hq", [(2, 8), (9, 64)])
+def test_short_units_one_after_the_other(t, hq):
+    """Segments of one KV tile, many to a CTA, in which one of the two streams has nothing to do; with longer ones between."""
+    lens = [1 + 7 * i % 128 for i in range(400)] + [128 * (1 + i % 3) - i % 2 for i in range(60)] + [5] * 40
+    s = make(lens, [min(n, t) for n in lens], [t] * len(lens), hq, hq // 8, 16, "HND", "fp16", seed=t)
+    first = check(s, "HND", "fp16", max_seq_len=384, max_q_len=t)
+    for _ in range(20):
+        again = attention.tree_decode(*s.values(), max_seq_len=384, max_q_len=t)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
 def test_long_sequence_and_shards_of_it():
     """The shards' outputs, combined, are the attention over the whole."""
     from helix_a2a_b200 import lse_combine
