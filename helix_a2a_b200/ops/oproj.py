@@ -28,7 +28,14 @@ def oproj(x: torch.Tensor, w, *, splits: int = 0, library: Optional[bool] = None
     overlap take about 3 us more).  So with ``splits=0`` and a plain weight matrix calls of 32 tokens or more go to
     ``torch.nn.functional.linear``; ``library=False`` (or ``HELIX_A2A_OPROJ_LIBRARY=0``) keeps the hand-written
     kernel for every size.  Packed weights always use the hand-written kernel (the plain matrix is not kept).
+
+    ``w`` may also be an :class:`Int4OprojWeight` (``splits`` and ``library`` have no meaning then): bf16 or fp16 ``x`` like its
+    scales, a quarter of the bytes.
     """
+    if isinstance(w, Int4OprojWeight):
+        if not x.is_cuda:
+            return (x.float() @ unpack_weight_int4(w).t()).to(x.dtype)
+        return _ext.ops().oproj_int4(x, w.packed, w.scales, w.zeros, w.hidden, w.K, w.group)
     if isinstance(w, PackedOprojWeight):
         if not x.is_cuda:
             return (x.float() @ unpack_weight(w).float().t()).to(x.dtype)
@@ -90,6 +97,78 @@ def unpack_weight(pw: PackedOprojWeight) -> torch.Tensor:
     c = torch.arange(8, device=t.device).view(1, 1, 1, 8, 1)
     t = torch.gather(t, 3, (c ^ (r & 7)).expand_as(t).contiguous())   # the swizzle is its own inverse
     return t.permute(0, 2, 1, 3, 4).reshape(pw.hidden, na * 64)[:, :pw.K].contiguous()
+
+
+class Int4OprojWeight:
+    """A ``[hidden, K]`` weight in 4 bits with one scale (and zero point) per row and ``group`` columns: ``(q - z) * s`` with ``q`` and
+    ``z`` in 0 .. 15, ``z = 8`` where there are no zero points.  Laid out for the kernel (``csrc/oproj_int4.h``): per 16 rows and 64
+    columns the nibbles of every lane's matrix operands, scales and zero points as pairs of rows ``g`` and ``g + 8``.  Made by
+    :func:`quantize_weight_int4` from a matrix or by :func:`pack_weight_int4` from a checkpoint's arrays, once, at load time."""
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], hidden: int, K: int, group: int):
+        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self.hidden, self.K, self.group = hidden, K, group
+
+    @property
+    def shape(self):
+        return (self.hidden, self.K)
+
+
+def _row_pairs(t: torch.Tensor) -> torch.Tensor:
+    """``[hidden, groups]`` -> ``[hidden / 16, groups, 8, 2]``: rows ``g`` and ``g + 8`` of 16 side by side."""
+    hidden, groups = t.shape
+    return t.view(hidden // 16, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
+
+
+def pack_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None) -> Int4OprojWeight:
+    """``qweight [hidden, K / 2]`` uint8 (column ``2 i`` in the low half of byte ``i``), ``scales [hidden, K / group]`` bf16 or fp16 and
+    ``zeros`` uint8 of the same shape (values 0 .. 15; ``None``: 8 everywhere) -> :class:`Int4OprojWeight`.  ``group`` is 32, 64 or 128."""
+    hidden, K = qweight.shape[0], 2 * qweight.shape[1]
+    group = K // max(scales.shape[-1], 1)
+    if qweight.dtype != torch.uint8 or scales.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("pack_weight_int4 needs uint8 nibbles and bfloat16 or float16 scales")
+    if group not in (32, 64, 128) or scales.shape != (hidden, K // group) or hidden % 16 or K % 64 or K % group or not hidden or not K:
+        raise ValueError("pack_weight_int4 needs hidden % 16 == 0, K % 64 == 0 and scales [hidden, K / group], group 32, 64 or 128")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise ValueError("zeros must be uint8 of the scales' shape")
+    q = torch.stack([qweight & 15, qweight >> 4], -1).view(hidden, K)
+    # row = 16 T + 8 r + g, column = 64 u + 32 c + 8 t + 4 o + 2 h + e (chunk, lane, step, half, element):
+    # word (c, o) of lane (g, t) has the nibble of register 2 h + r at 2 h + r, + 4 for the odd column
+    q = q.view(hidden // 16, 2, 8, K // 64, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)    # T u g t c o e h r
+    q = q.reshape(hidden // 16, K // 64, 32, 4, 4, 2)
+    packed = (q[..., 0] | (q[..., 1] << 4)).contiguous().view(-1)
+    return Int4OprojWeight(packed, _row_pairs(scales), None if zeros is None else _row_pairs(zeros), hidden, K, group)
+
+
+def quantize_weight_int4(w: torch.Tensor, group: int = 128, *, zero_points: bool = False) -> Int4OprojWeight:
+    """Round a bf16 or fp16 ``[hidden, K]`` matrix to 4 bits, to the nearest: with zero points a group's range from its least to its
+    largest value (and zero), without them -7 .. 7 times its largest magnitude / 7.  The scales have the matrix's type."""
+    if w.dtype not in (torch.bfloat16, torch.float16) or w.dim() != 2 or group not in (32, 64, 128) or w.shape[1] % group or w.shape[1] % 64 \
+            or w.shape[0] % 16:
+        raise ValueError("quantize_weight_int4 needs a bfloat16 or float16 [hidden % 16 == 0, K % 64 == 0 and % group == 0] matrix")
+    hidden, K = w.shape
+    v = w.float().view(hidden, K // group, group)
+    least = 2.0 ** -24                                   # a group of zeros has to have a scale, too
+    if zero_points:
+        lo, hi = v.amin(-1).clamp(max=0), v.amax(-1).clamp(min=0)
+        scales = ((hi - lo) / 15).clamp(min=least).to(w.dtype)
+        zeros = (-lo / scales.float()).round().clamp(0, 15)
+    else:
+        scales = (v.abs().amax(-1) / 7).clamp(min=least).to(w.dtype)
+        zeros = torch.full_like(scales, 8, dtype=torch.float32)
+    q = (v / scales.float().unsqueeze(-1) + zeros.unsqueeze(-1)).round().clamp(0, 15).to(torch.uint8).view(hidden, K)
+    return pack_weight_int4(q[:, 0::2] | (q[:, 1::2] << 4), scales, zeros.to(torch.uint8) if zero_points else None)
+
+
+def unpack_weight_int4(w: Int4OprojWeight) -> torch.Tensor:
+    """The fp32 ``[hidden, K]`` matrix that a packed 4-bit weight stands for (oracles, debugging)."""
+    q = torch.stack([w.packed & 15, w.packed >> 4], -1).view(w.hidden // 16, w.K // 64, 8, 4, 2, 2, 2, 2, 2)   # T u g t c o e h r
+    q = q.permute(0, 8, 2, 1, 4, 3, 5, 7, 6).reshape(w.hidden, w.K // w.group, w.group).float()
+
+    def rows(t):
+        return t.permute(0, 3, 2, 1).reshape(w.hidden, -1, 1).float()
+
+    return ((q - (8.0 if w.zeros is None else rows(w.zeros))) * rows(w.scales)).view(w.hidden, w.K)
 
 
 def check_compute_status(like: torch.Tensor) -> None:
