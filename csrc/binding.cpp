@@ -382,7 +382,6 @@ torch::Tensor read_status(torch::Tensor workspace, int64_t cp_rank, int64_t cp_s
 void register_compute_ops(torch::Library& m);
 void bind_compute(pybind11::module_& m);
 void register_paged_ops(torch::Library& m);
-void register_int4_ops(torch::Library& m);
 
 TORCH_LIBRARY(helix_a2a_b200, m) {
   m.def("get_helix_workspace_size_per_rank(int cp_size) -> int", &get_helix_workspace_size_per_rank);
@@ -405,7 +404,6 @@ TORCH_LIBRARY(helix_a2a_b200, m) {
         &lse_combine);
   register_compute_ops(m);
   register_paged_ops(m);
-  register_int4_ops(m);
 }
 
 // ---- pybind module: allocator + host utilities ---------------------------------------------------

@@ -15,6 +15,7 @@
 #include "fifo.cuh"
 #include "fused.h"
 #include "oproj.h"
+#include "oproj_int4.h"
 #include "tensor_map.h"
 #include "tree_attn.h"
 
@@ -532,6 +533,52 @@ torch::Tensor oproj_packed(torch::Tensor x, torch::Tensor packed, int64_t hidden
   return y;
 }
 
+// ---- o_proj with 4-bit weights ------------------------------------------------------------------------
+// x [tokens, K]; packed: uint8 [slabs of 128 rows, bytes] as made by helix_a2a_b200.ops.oproj.pack_weight_int4, whose scales had x's type
+torch::Tensor oproj_int4(torch::Tensor x, torch::Tensor packed, int64_t hidden, int64_t K, int64_t group, bool zeros) {
+  TORCH_CHECK(x.is_cuda(), "inputs must be on CUDA");
+  const torch::Device dev = x.device();
+  TORCH_CHECK(packed.device() == dev, "x and the weight must be on one device");
+  const auto type = x.scalar_type();
+  TORCH_CHECK(type == at::ScalarType::BFloat16 || type == at::ScalarType::Half, "x must be bfloat16 or float16");
+  TORCH_CHECK(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
+  TORCH_CHECK(hidden > 0 && K > 0 && K % 64 == 0 && K % group == 0, "K must be a multiple of 64 and of the group");
+  TORCH_CHECK(K <= 0x7fffff00 && hidden <= 0x7fffff00, "hidden and K are counted in 32 bits");
+  TORCH_CHECK(x.dim() == 2 && x.size(1) == K && x.stride(1) == 1, "x must be [tokens, K]");
+  const int64_t tokens = x.size(0);
+  TORCH_CHECK(tokens == 0 || (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && (tokens == 1 || x.stride(0) % 8 == 0)),
+              "rows of x must start on 16-byte boundaries");
+  TORCH_CHECK(packed.scalar_type() == at::ScalarType::Byte && packed.is_contiguous() &&
+                  (size_t)packed.numel() == (hidden + 127) / 128 * helix::int4_slab_bytes(K, group, zeros) &&
+                  reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 == 0,
+              "packed weight has the wrong size or alignment for [", hidden, ", ", K, "] in groups of ", group);
+  c10::cuda::CUDAGuard guard(dev);
+  auto stream = at::cuda::getCurrentCUDAStream();
+  torch::Tensor y = torch::empty({tokens, hidden}, x.options());
+  if (tokens == 0) return y;
+  ScratchUse sc = scratch_for(dev, false, 0, 0, 0);
+  for (int64_t t0 = 0; t0 < tokens; t0 += helix::kInt4MaxTokens) {
+    helix::OprojInt4Params p{};
+    p.tokens = (int)std::min<int64_t>(tokens - t0, helix::kInt4MaxTokens);
+    const uint64_t dims[2] = {(uint64_t)K, (uint64_t)p.tokens}, strides[1] = {(uint64_t)(p.tokens > 1 ? x.stride(0) : K) * 2};
+    const uint32_t box[2] = {64, (uint32_t)helix::int4_pad_tokens(p.tokens)};
+    const char* err = nullptr;
+    TORCH_CHECK(helix::encode_tensor_map(&p.x_map, type == at::ScalarType::Half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                                         reinterpret_cast<uint16_t*>(x.data_ptr()) + t0 * x.stride(0), dims, strides, box, helix::TmaSwizzle::k128B, &err),
+                "helix: activation tensor map: ", err ? err : "?");
+    p.w = packed.data_ptr<uint8_t>();
+    p.y = reinterpret_cast<uint16_t*>(y.data_ptr()) + t0 * hidden;
+    p.y_stride = hidden;
+    p.error_flag = sc.dev.error_flag.data_ptr<int32_t>();
+    p.timeout_ns = env_timeout_ns();
+    p.hidden = (int)hidden; p.K = (int)K; p.group = (int)group;
+    p.zeros = zeros;
+    p.is_bf16 = type == at::ScalarType::BFloat16;
+    check_cuda(helix::launch_oproj_int4(p, env_pdl(), helix::device_sm_count(), stream), "o_proj (4-bit) launch");
+  }
+  return y;
+}
+
 torch::Tensor attn_trace(torch::Tensor like) {
   ScratchUse sc = scratch_for(like.device(), false, 1, 0, 0);
   TORCH_CHECK(sc.dev.trace.defined(), "no trace recorded: set HELIX_A2A_ATTN_TRACE=1 (or HELIX_A2A_OPROJ_TRACE=1)");
@@ -710,6 +757,7 @@ void register_compute_ops(torch::Library& m) {
       "float scale, bool lse_base2, int ctas, int max_seq_len) -> (Tensor, Tensor)",
       &mla_decode);
   m.def("oproj(Tensor x, Tensor w, int splits) -> Tensor", &oproj);
+  m.def("oproj_int4(Tensor x, Tensor packed, int hidden, int K, int group, bool zeros) -> Tensor", &oproj_int4);
   m.def("oproj_packed(Tensor x, Tensor packed, int hidden, int K, int splits) -> Tensor", &oproj_packed);
   m.def(
       "alltoall_combine_oproj(Tensor attn_out, Tensor lse, Tensor w, Tensor workspace, int cp_rank, int cp_size, bool "

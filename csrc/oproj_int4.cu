@@ -1,20 +1,25 @@
-// o_proj with 4-bit weights for few tokens: a matrix-vector product on the warp-level tensor-core MMA.
+// o_proj with 4-bit weights: a GEMM whose weights become tensor-core operands on the way.
 //
-// Bound by streaming the weights once (8192 x 8192: 33.5 MB, 5.1 us at the copy rate).  Everything is arranged so that a
-// weight costs one pass through registers:
-//   * A warp owns 256 columns, whose x it holds in registers as MMA B operands for the whole launch, and walks over 16-row tiles.  The
-//     packed layout hands every lane its A operand as words of eight nibbles; with 0x4300 in front (0x6400 for fp16) a nibble is the
-//     number 128 + q (1024 + q), from which 128 + z is subtracted exactly: three instructions for two weights.
-//   * The products of a group are summed by the MMA in fp32 from exact integers, and only their sum is multiplied by the scale.
-//   * The warps of a CTA, and up to eight CTAs of a cluster, share out the columns.  Their sums meet in shared memory, by distributed
-//     shared memory across the cluster: no scratch memory, no atomics, one launch, one order of summation.
-//   * Weights of the next tiles are requested before the present one is used; the first ones before the preceding kernel is waited for.
+// Bound by streaming the weights once for a few tokens (8192 x 8192: 33.5 MB, 5.1 us at the copy rate), by the tensor cores only beyond
+// some hundred.  A CTA owns 128 rows (a slab, M of the MMA) and a run of columns; tokens are the MMA's N.
+//   * Records of the packed weight arrive by bulk copy.  Eight warps turn nibbles into numbers: with 0x4300 in front (0x6400 for fp16) a
+//     nibble is 128 + q (1024 + q), from which 128 + z is subtracted exactly; 16 bytes go into the swizzled A operand at a time.
+//   * tcgen05 sums each group's products in fp32 from these exact integers, into one of a few accumulators in tensor memory.  The
+//     same eight warps, a thread per row (and half of the tokens), fetch a finished group and add it, times its scale, to their sums in registers:
+//     scales and zero points cost no rounding, which folding them into 16-bit weights would (half a step per weight).
+//   * The CTAs of a cluster share out a slab's columns and send each other their sums through distributed shared memory, each finishing
+//     a part of the rows: no scratch memory, no atomics, one launch, one order of summation.
+// The same product on warp-level MMAs, weights in registers, took 13.4 us for 8 tokens (8192 x 8192) and 126 us for 100 (7168 x 8192): they
+// cost ~16 cycles per 256 weights and 8 tokens.
 #include "oproj_int4.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <map>
+#include <mutex>
+#include <tuple>
 
 #include "helix_common.cuh"
 #include "sm100.cuh"
@@ -24,10 +29,25 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kUnits = 4;                 // 64-column units per warp
-constexpr int kMaxWarps = 16;
-constexpr int kBatch = 8;                 // row tiles whose sums a CTA keeps before it adds them up
-constexpr int kAhead = 2;                 // tiles requested ahead
+constexpr int kRows = 128;
+constexpr int kWorkers = 8, kMmaWarp = 8, kThreads = 320;        // and a warp that loads
+constexpr int kBlockBytes = kRows * 128;               // A operand of 64 columns
+constexpr int kStages = 4;                             // records of 128 columns on their way
+constexpr int kNibbles = 4096;                         // bytes of a block of 64 columns
+constexpr int kMaxRecord = 2 * kNibbles + 4 * 384;     // 128 columns in groups of 32, with zero points
+constexpr int kMaxCluster = 8;
+
+template <int N>
+struct Shape {
+  static constexpr int ctas = N <= 64 ? 2 : 1;         // per SM
+  static constexpr int slots = N <= 64 ? 3 : 4;        // operand blocks between dequantisation and MMA
+  static constexpr int accs = 4;                       // accumulators in tensor memory
+  static constexpr int cols = accs * N;
+  static constexpr int x_bytes = N * 128;              // B operand of 64 columns
+  static constexpr int ring = slots * (kBlockBytes + x_bytes) + kStages * kMaxRecord;
+  static constexpr int row = N * 4 + 16;               // bytes between rows of sums that CTAs send each other
+  static constexpr int smem = ring + 1024;
+};
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
@@ -38,209 +58,279 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (BF16) {
-    mma_bf16_16816(c, a[0], a[1], a[2], a[3], b0, b1);
-  } else {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
 template <bool BF16>
-__device__ __forceinline__ float2 widen2(uint32_t x) {
-  if (BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+__device__ __forceinline__ float widen(uint16_t x) {
+  return BF16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
 }
-__device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+template <bool BF16>
+__device__ __forceinline__ uint16_t narrow(float x) {
+  return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
 }
 
-// NT: tiles of eight tokens
-template <bool BF16, int NT, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(kMaxWarps * 32, 1) oproj_int4_kernel(const __grid_constant__ OprojInt4Params p) {
-  constexpr int kGroups = kUnits * 64 / GROUP;         // of a warp's columns
-  constexpr int kSum = 16 * 8 * NT;                    // sums of one row tile
-  extern __shared__ float s_sum[];                     // [warps][kBatch][kSum], behind it [kBatch][kSum] of the whole CTA
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int warps = blockDim.x >> 5, cl = (int)(gridDim.y), rank = (int)blockIdx.y;      // a cluster is a column of the grid
-  const int units = p.K / 64, unit0 = (rank * warps + warp) * kUnits;
-  const int n_units = min(max(units - unit0, 0), kUnits);
-  const int tiles = p.hidden / 16, n_groups = p.K / GROUP;
-  struct Tile {
-    uint4 w[kUnits];
-    uint32_t s[kGroups];
-    uint32_t z[ZEROS ? kGroups : 1];
-  };
-  auto fetch = [&](int tile, Tile& f) {
-    const uint4* w = p.w + ((int64_t)tile * units + unit0) * 32 + lane;
-    const int64_t s0 = ((int64_t)tile * n_groups + unit0 * 64 / GROUP) * 8 + g;
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) f.w[u] = tile < tiles && u < n_units ? ldg_stream(w + u * 32) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      const bool in = tile < tiles && i * GROUP < n_units * 64;
-      f.s[i] = in ? __ldg(p.scales + s0 + i * 8) : 0u;
-      if (ZEROS) f.z[i] = in ? __ldg(p.zeros + s0 + i * 8) : 0u;
+template <bool BF16, int N>
+__global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(const __grid_constant__ OprojInt4Params p) {
+  using S = Shape<N>;
+  constexpr int NH = N / 2;                            // tokens of a worker thread
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t w_full[kStages], w_free[kStages], a_full[S::slots], x_full[S::slots], a_free[S::slots], d_full[S::accs],
+      d_free[S::accs], drain;
+  __shared__ uint32_t tmem_slot;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* const a_ring = smem;
+  uint8_t* const x_ring = smem + S::slots * kBlockBytes;
+  uint8_t* const w_ring = x_ring + S::slots * S::x_bytes;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cl = (int)gridDim.y, rank = (int)blockIdx.y, slab = (int)blockIdx.x;          // a cluster is a column of the grid
+  const int records = (p.K + 127) / 128, r0 = (int)((int64_t)records * rank / cl), r1 = (int)((int64_t)records * (rank + 1) / cl);
+  const int b0 = 2 * r0, blocks = min(2 * r1, p.K / 64) - b0;        // of 64 columns
+  const int group = p.group, group_bytes = p.zeros ? 384 : 256;
+
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&w_full[i], 1);
+      mbar_init(&w_free[i], kWorkers);
     }
-  };
-  Tile ahead[kAhead];
-  const int step = gridDim.x;
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) fetch(blockIdx.x + i * step, ahead[i]);
+    for (int i = 0; i < S::slots; ++i) {
+      mbar_init(&a_full[i], kWorkers);
+      mbar_init(&x_full[i], 1);
+      mbar_init(&a_free[i], 1);
+    }
+    for (int i = 0; i < S::accs; ++i) {
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_free[i], kWorkers);
+    }
+    mbar_init(&drain, 1);
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&tmem_slot, S::cols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  const unsigned long long deadline = now_ns() + p.timeout_ns;
+  bool ok = true;
 
+  float acc[NH];
+#pragma unroll
+  for (int j = 0; j < NH; ++j) acc[j] = 0.f;
+  if (warp < kWorkers) {
+    // =========================== dequantisation, and the sums ===========================
+    const int row = tid & (kRows - 1), half = tid >> 7;              // 32 of a block's columns; half of the tokens
+    const uint32_t tq = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * NH;
+    // both in registers: with two constants the compiler makes two instructions of (w & mask) | magic
+    uint32_t mask, magic;
+    asm volatile("mov.u32 %0, 0x000f000f;" : "=r"(mask));
+    asm volatile("mov.u32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300 : 0x64006400));
+    int n_done = 0;                                                  // groups added up so far
+    float s_now[2] = {0.f, 0.f}, s_last[2];                          // scales of this block's groups and of the one before
+    int ends_now = 0, ends_last;                                     // groups that end with the block
+    auto add_groups = [&](int n, const float (&s)[2]) {
+      for (int i = 0; i < n && ok; ++i, ++n_done) {
+        const int d = n_done % S::accs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (n_done / S::accs) & 1, deadline));
+        if (!ok) break;
+        tc_fence_after_sync();
+        uint32_t v[NH];
+        if constexpr (NH == 8) tmem_ld_x8(tq + d * N, v);
+        else if constexpr (NH == 16) tmem_ld_32x32b_x16(tq + d * N, v);
+        else if constexpr (NH == 32) tmem_ld_x32(tq + d * N, v);
+        else {
+          tmem_ld_x32(tq + d * N, *reinterpret_cast<uint32_t(*)[32]>(v));
+          tmem_ld_x32(tq + d * N + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+        }
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&d_free[d]);
+        const float sc = i == 0 ? s[0] : s[1];
+#pragma unroll
+        for (int j = 0; j < NH; ++j) acc[j] += sc * __uint_as_float(v[j]);
+      }
+    };
+    for (int b = 0; b < blocks && ok; ++b) {
+      const int rec = b >> 1, st = rec % kStages, sl = b % S::slots;
+      const int in_record = min(2, blocks - 2 * rec) * 64, col = (b & 1) * 64;           // columns of the record; the block's first
+      if ((b & 1) == 0) ok = __all_sync(0xffffffffu, mbar_wait(&w_full[st], (rec / kStages) & 1, deadline));
+      if (ok && b >= S::slots) ok = __all_sync(0xffffffffu, mbar_wait(&a_free[sl], (b / S::slots - 1) & 1, deadline));
+      if (!ok) break;
+      const uint8_t* w = w_ring + st * kMaxRecord;
+      const uint4 q = *reinterpret_cast<const uint4*>(w + (b & 1) * kNibbles + half * (kRows * 16) + row * 16);
+      const uint8_t* scales = w + in_record * 64;
+      const uint32_t z = p.zeros ? scales[in_record / group * 256 + (col + 32 * half) / group * kRows + row] : 8u;
+      const uint32_t z2 = magic + (z & 0xfu) * 0x00010001u;          // 128 + z, twice
+      s_last[0] = s_now[0], s_last[1] = s_now[1];
+      ends_last = ends_now;
+      ends_now = group == 32 ? 2 : group == 64 ? 1 : b & 1;
+      s_now[0] = widen<BF16>(reinterpret_cast<const uint16_t*>(scales + col / group * 256)[row]);
+      s_now[1] = group == 32 ? widen<BF16>(reinterpret_cast<const uint16_t*>(scales + (col / group + 1) * 256)[row]) : 0.f;
+      const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+      uint8_t* a = a_ring + sl * kBlockBytes;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = sub2<BF16>(and_or(words[c] >> (4 * i), mask, magic), z2);
+        *reinterpret_cast<uint4*>(a + swz128(row, 4 * half + c)) = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&a_full[sl]);
+        if ((b & 1) == 1 || b + 1 == blocks) mbar_arrive(&w_free[st]);
+      }
+      add_groups(ends_last, s_last);
+    }
+    if (ok) add_groups(ends_now, s_now);
+  } else if (warp == kMmaWarp) {
+    // =========================== MMA issue ===========================
+    constexpr uint32_t idesc = BF16 ? umma_idesc_bf16(kRows, N) : umma_idesc_bf16(kRows, N) & ~((1u << 7) | (1u << 10));
+    const uint64_t d_a = umma_desc_k_sw128(smem_u32(a_ring)), d_x = umma_desc_k_sw128(smem_u32(x_ring));
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0; };
+    uint32_t n_group = 0;
+    for (int b_lane = 0; b_lane < blocks && ok; ++b_lane) {
+      // the block number through a shuffle: what is computed from it is then known to be the same in all lanes
+      const int b = __shfl_sync(0xffffffffu, b_lane, 0), sl = b % S::slots;
+      ok = wait(&x_full[sl], (b / S::slots) & 1) && wait(&a_full[sl], (b / S::slots) & 1);
+      for (int k0 = 0; k0 < 64 && ok; k0 += 32) {
+        const uint32_t n = __shfl_sync(0xffffffffu, n_group, 0), d = n % S::accs;
+        const bool first = (b * 64 + k0) % group == 0, last = (b * 64 + k0 + 32) % group == 0;
+        if (first && n >= (uint32_t)S::accs) ok = wait(&d_free[d], (n / S::accs - 1) & 1);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const uint32_t off = k0 * 2 + ks * 32;
+            umma_bf16(tmem + d * N, d_a + ((sl * kBlockBytes + off) >> 4), d_x + ((sl * S::x_bytes + off) >> 4), idesc, !(first && ks == 0));
+          }
+          if (last) umma_commit(&d_full[d]);
+          if (k0 == 32) umma_commit(&a_free[sl]);
+        }
+        __syncwarp();
+        n_group += last;
+      }
+    }
+    // the last commits have to arrive before this CTA leaves
+    for (int b = max(0, blocks - S::slots); b < blocks && ok; ++b) ok = wait(&a_free[b % S::slots], (b / S::slots) & 1);
+    if (!ok) {
+      if (elect_one()) umma_commit(&drain);            // nothing of this CTA's may be in flight when it leaves
+      mbar_wait(&drain, 0, now_ns() + 10000000ull);
+    }
+  } else {
+    // =========================== loads ===========================
+    const uint8_t* w = p.w + (int64_t)slab * (int64_t)((int64_t)p.K * 64 + p.K / group * group_bytes) + (int64_t)r0 * (128 * 64 + 128 / group * group_bytes);
+    const int n_rec = r1 - r0;
+    int w_at = 0, x_at = 0;
+    auto load_w = [&]() {
+      const int st = w_at % kStages, cols = min(2, blocks - 2 * w_at) * 64;
+      if (w_at >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&w_free[st], (w_at / kStages - 1) & 1, deadline));
+      if (!ok) return;
+      const uint32_t bytes = cols * 64 + cols / group * group_bytes;
+      if (lane == 0) {
+        mbar_expect_tx(&w_full[st], bytes);
+        bulk_load_1d(w_ring + st * kMaxRecord, w + (int64_t)w_at * (128 * 64 + 128 / group * group_bytes), bytes, &w_full[st]);
+      }
+      __syncwarp();
+      ++w_at;
+    };
+    while (w_at < min(n_rec, kStages) && ok) load_w();               // weights do not depend on the kernel before this one
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    while (x_at < blocks && ok) {
+      const int sl = x_at % S::slots;
+      if (x_at >= S::slots) ok = __all_sync(0xffffffffu, mbar_wait(&a_free[sl], (x_at / S::slots - 1) & 1, deadline));
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(&x_full[sl], S::x_bytes);
+        tma_load_2d(x_ring + sl * S::x_bytes, &p.x_map, &x_full[sl], (b0 + x_at) * 64, 0);
+      }
+      __syncwarp();
+      ++x_at;
+      // a record's place is free when its last block has been dequantised, long before that block's x is used
+      if ((x_at & 1) == 0 && w_at < n_rec) load_w();
+    }
+    while (w_at < n_rec && ok) load_w();
+    if (!ok) {
+      // nothing may land in this CTA's shared memory after it has left
+      const unsigned long long limit = now_ns() + 10000000ull;
+      for (int i = max(0, w_at - kStages); i < w_at; ++i) mbar_wait(&w_full[i % kStages], (i / kStages) & 1, limit);
+      for (int i = max(0, x_at - S::slots); i < x_at; ++i) mbar_wait(&x_full[i % S::slots], (i / S::slots) & 1, limit);
+    }
+  }
+  if (!ok && lane == 0) atomicCAS(p.error_flag, 0, (int)kTimeoutMbarrier);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  uint32_t x[NT][kUnits][8];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int n = nt * 8 + g;
-    const uint4* row = reinterpret_cast<const uint4*>(p.x + n * p.x_stride + unit0 * 64 + 8 * t);
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint4 v = n < p.tokens && u < n_units ? __ldg(row + u * 8 + c * 4) : make_uint4(0, 0, 0, 0);
-        x[nt][u][4 * c] = v.x, x[nt][u][4 * c + 1] = v.y, x[nt][u][4 * c + 2] = v.z, x[nt][u][4 * c + 3] = v.w;
-      }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, S::cols);
   }
 
-  float* const mine = s_sum + warp * (kBatch * kSum);
-  float* const whole = s_sum + warps * (kBatch * kSum);
-  constexpr uint32_t kMagic = BF16 ? 0x43004300u : 0x64006400u;
-  for (int tile0 = blockIdx.x; tile0 < tiles; tile0 += kBatch * step) {
-    const int batch = min(kBatch, (tiles - tile0 + step - 1) / step);
-#pragma unroll 2
-    for (int j = 0; j < batch; ++j) {
-      const Tile f = ahead[0];
+  // ---- results: thread (row, half) holds tokens half * NH ... of its row ----------------------------------
+  const int row = tid & (kRows - 1), half = tid >> 7;
+  const int rows_here = min(kRows, p.hidden - slab * kRows);
+  if (cl == 1) {
+    if (warp < kWorkers && row < rows_here) {
 #pragma unroll
-      for (int i = 0; i + 1 < kAhead; ++i) ahead[i] = ahead[i + 1];
-      fetch(tile0 + (j + kAhead) * step, ahead[kAhead - 1]);
-      float acc[NT][4], part[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const uint32_t w[4] = {f.w[u].x, f.w[u].y, f.w[u].z, f.w[u].w};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const int k = u * 64 + s * 16, grp = k / GROUP;
-          if (k % GROUP == 0) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) part[nt][i] = 0.f;
-          }
-          // 128 + z of rows g and g + 8, twice each
-          uint32_t z0 = kMagic + 0x00080008u, z1 = z0;
-          if (ZEROS) {
-            z0 = kMagic + (f.z[grp] & 0xfu) * 0x00010001u;
-            z1 = kMagic + (f.z[grp] >> 8 & 0xfu) * 0x00010001u;
-          }
-          uint32_t a[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] = sub2<BF16>((w[s] >> (4 * i) & 0x000f000fu) | kMagic, i & 1 ? z1 : z0);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<BF16>(part[nt], a, x[nt][u][2 * s], x[nt][u][2 * s + 1]);
-          if ((k + 16) % GROUP == 0) {
-            const float2 sc = widen2<BF16>(f.s[grp]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              acc[nt][0] += sc.x * part[nt][0];
-              acc[nt][1] += sc.x * part[nt][1];
-              acc[nt][2] += sc.y * part[nt][2];
-              acc[nt][3] += sc.y * part[nt][3];
-            }
-          }
-        }
-      }
-      // [token][row], tokens 2 t and 2 t + 1
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float* to = mine + j * kSum + (nt * 8 + 2 * t) * 16 + g;
-        to[0] = acc[nt][0];
-        to[16] = acc[nt][1];
-        to[8] = acc[nt][2];
-        to[24] = acc[nt][3];
+      for (int j = 0; j < NH; ++j) {
+        const int n = half * NH + j;
+        if (n < p.tokens) p.y[n * p.y_stride + slab * kRows + row] = narrow<BF16>(acc[j]);
       }
     }
-    __syncthreads();
-    // the warps' sums, in the order of the columns
-    for (int e = threadIdx.x; e < batch * kSum; e += blockDim.x) {
-      float v = s_sum[e];
-      for (int w = 1; w < warps; ++w) v += s_sum[w * (kBatch * kSum) + e];
-      whole[e] = v;
-    }
-    auto store = [&](int e, float v) {
-      const int j = e / kSum, n = e % kSum / 16, r = e % 16;
-      if (n >= p.tokens) return;
-      uint16_t* to = p.y + n * p.y_stride + (int64_t)(tile0 + j * step) * 16 + r;
-      if (BF16) *reinterpret_cast<__nv_bfloat16*>(to) = __float2bfloat16_rn(v);
-      else *reinterpret_cast<__half*>(to) = __float2half_rn(v);
-    };
-    if (cl == 1) {
-      for (int e = threadIdx.x; e < batch * kSum; e += blockDim.x) store(e, whole[e]);
-      __syncthreads();
-    } else {
-      __syncwarp();
-      cluster_arrive();
-      cluster_wait();
-      // rank r finishes runs of 32 sums
-      for (int e = rank * 32 + (threadIdx.x & 31) + warp * 32 * cl; e < batch * kSum; e += blockDim.x * cl) {
-        float v = 0.f;
-        for (int c = 0; c < cl; ++c) v += ld_cluster_f32(map_to_cta(smem_u32(whole + e), c));
-        store(e, v);
-      }
-      __syncwarp();
-      cluster_arrive();                                // nobody leaves, or begins the next batch, while a peer reads
-      cluster_wait();
-    }
+    return;
+  }
+  // Rank r finishes rows r * per ... of the slab.  Everybody is through with its rings, so they take the others' sums.
+  const int per = (kRows / 8 + cl - 1) / cl * 8;
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (warp < kWorkers) {
+    const uint32_t to = map_to_cta(smem_u32(smem) + (rank * per + row % per) * S::row + half * NH * 4, row / per);
+#pragma unroll
+    for (int j = 0; j < NH; j += 4) st_cluster_f32x4(to + j * 4, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+  }
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  const int mine = max(min(per, rows_here - rank * per), 0);
+  for (int e = tid; e < per * p.tokens; e += kThreads) {
+    const int n = e / per, r = e % per;
+    if (r >= mine) continue;
+    const uint8_t* from = smem + r * S::row + n * 4;
+    float v = *reinterpret_cast<const float*>(from);
+    for (int c = 1; c < cl; ++c) v += *reinterpret_cast<const float*>(from + c * per * S::row);
+    p.y[n * p.y_stride + slab * kRows + rank * per + r] = narrow<BF16>(v);
   }
 }
 
 using Fn = void (*)(OprojInt4Params);
-template <bool BF16, int NT>
-Fn pick(int group, bool zeros) {
-  if (group == 32) return zeros ? (Fn)oproj_int4_kernel<BF16, NT, 32, true> : (Fn)oproj_int4_kernel<BF16, NT, 32, false>;
-  if (group == 64) return zeros ? (Fn)oproj_int4_kernel<BF16, NT, 64, true> : (Fn)oproj_int4_kernel<BF16, NT, 64, false>;
-  return zeros ? (Fn)oproj_int4_kernel<BF16, NT, 128, true> : (Fn)oproj_int4_kernel<BF16, NT, 128, false>;
+template <bool BF16>
+Fn pick(int n, size_t* smem) {
+  if (n == 16) return *smem = Shape<16>::smem, (Fn)oproj_int4_kernel<BF16, 16>;
+  if (n == 32) return *smem = Shape<32>::smem, (Fn)oproj_int4_kernel<BF16, 32>;
+  if (n == 64) return *smem = Shape<64>::smem, (Fn)oproj_int4_kernel<BF16, 64>;
+  return *smem = Shape<128>::smem, (Fn)oproj_int4_kernel<BF16, 128>;
 }
 
-}  // namespace
-
-cudaError_t launch_oproj_int4(const OprojInt4Params& p, bool pdl, int sm_count, cudaStream_t stream) {
-  if (p.tokens <= 0 || p.hidden <= 0) return cudaSuccess;
-  if (p.tokens > kInt4MaxTokens || p.K <= 0 || p.K > kInt4MaxK || p.K % 64 != 0 || p.hidden % 16 != 0 ||
-      (p.group != 32 && p.group != 64 && p.group != 128) || p.K % p.group != 0)
-    return cudaErrorInvalidValue;
-  const int units = p.K / 64, slices = (units + kUnits - 1) / kUnits, nt = (p.tokens + 7) / 8;
-  int cl = 1;
-  while (slices > cl * kMaxWarps) cl *= 2;
-  const int warps = (slices + cl - 1) / cl;
-  const int tiles = p.hidden / 16, columns = std::max(sm_count * (kMaxWarps / warps) / cl, 1);
-  const Fn fn = p.is_bf16 ? (nt == 1 ? pick<true, 1>(p.group, p.zeros != nullptr) : pick<true, 2>(p.group, p.zeros != nullptr))
-                          : (nt == 1 ? pick<false, 1>(p.group, p.zeros != nullptr) : pick<false, 2>(p.group, p.zeros != nullptr));
-  const size_t smem = (size_t)(warps + 1) * kBatch * 16 * 8 * nt * sizeof(float);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
+cudaLaunchConfig_t config(int slabs, int cl, size_t smem, bool pdl, cudaStream_t stream, cudaLaunchAttribute (&attrs)[2]) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)std::min(tiles, columns), (unsigned)cl, 1);
-  cfg.blockDim = dim3((unsigned)warps * 32, 1, 1);
+  cfg.gridDim = dim3((unsigned)slabs, (unsigned)cl, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeClusterDimension;
   attrs[0].val.clusterDim.x = 1;
   attrs[0].val.clusterDim.y = (unsigned)cl;
@@ -249,6 +339,66 @@ cudaError_t launch_oproj_int4(const OprojInt4Params& p, bool pdl, int sm_count, 
   attrs[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attrs;
   cfg.numAttrs = pdl ? 2 : 1;
+  return cfg;
+}
+
+// Clusters of each size that are resident together, asked once per kernel and device
+struct Resident {
+  int clusters[kMaxCluster + 1];
+};
+cudaError_t resident(const void* fn, int dev, size_t smem, int sm_count, Resident* out) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, const void*>, Resident> known;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto key = std::make_tuple(dev, fn);
+  const auto it = known.find(key);
+  if (it != known.end()) {
+    *out = it->second;
+    return cudaSuccess;
+  }
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  Resident r{};
+  for (int cl = 1; cl <= kMaxCluster; ++cl) {
+    cudaLaunchAttribute attrs[2];
+    const cudaLaunchConfig_t cfg = config(sm_count, cl, smem, false, nullptr, attrs);
+    e = cudaOccupancyMaxActiveClusters(&r.clusters[cl], fn, &cfg);
+    if (e != cudaSuccess) return e;
+  }
+  known[key] = r;
+  *out = r;
+  return cudaSuccess;
+}
+
+}  // namespace
+
+cudaError_t launch_oproj_int4(const OprojInt4Params& p, bool pdl, int sm_count, cudaStream_t stream) {
+  if (p.tokens <= 0 || p.hidden <= 0) return cudaSuccess;
+  if (p.tokens > kInt4MaxTokens || p.K <= 0 || p.K % 64 != 0 || (p.group != 32 && p.group != 64 && p.group != 128) || p.K % p.group != 0)
+    return cudaErrorInvalidValue;
+  size_t smem = 0;
+  const int n = int4_pad_tokens(p.tokens);
+  const Fn fn = p.is_bf16 ? pick<true>(n, &smem) : pick<false>(n, &smem);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  Resident r;
+  cudaError_t e = resident((const void*)fn, dev, smem, sm_count, &r);
+  if (e != cudaSuccess) return e;
+  // As many CTAs per slab as make the launch shortest: rounds of resident clusters times the records of a CTA, and about three records'
+  // time for a CTA's start, the exchange and the end.
+  const int slabs = (p.hidden + kRows - 1) / kRows, records = (p.K + 127) / 128;
+  int best = 1;
+  int64_t cost = INT64_MAX;
+  for (int cl = 1; cl <= std::min(kMaxCluster, records); ++cl) {
+    if (r.clusters[cl] < 1) continue;
+    const int64_t c = (int64_t)((slabs + r.clusters[cl] - 1) / r.clusters[cl]) * ((records + cl - 1) / cl + 3);
+    if (c < cost) {
+      cost = c;
+      best = cl;
+    }
+  }
+  cudaLaunchAttribute attrs[2];
+  const cudaLaunchConfig_t cfg = config(slabs, best, smem, pdl, stream, attrs);
   return cudaLaunchKernelEx(&cfg, fn, p);
 }
 

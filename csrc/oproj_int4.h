@@ -1,6 +1,7 @@
-// o_proj with 4-bit weights and group scales: host interface (kernels in oproj_int4.cu).
+// o_proj with 4-bit weights and group scales: host interface (kernel in oproj_int4.cu).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -8,24 +9,24 @@ namespace helix {
 
 // y[n, r] = sum_k x[n, k] (q[r, k] - z[r, k / group]) s[r, k / group], q and z in 0 .. 15 (no zero points: z = 8).
 //
-// Packed weights: per 16 rows and 64 columns 512 bytes, 16 for each lane of a warp, four words of eight nibbles, one word per
-// 16 x 16 x 8 MMA.  Nibbles i and i + 4 of word s of lane (g, t) are the A operand's register i:
-//   row g + 8 (i & 1), columns k and k + 1,  k = 32 (s >> 1) + 8 t + 4 (s & 1) + 2 (i >> 1)
-// so that a lane's B operands of 32 columns are 16 consecutive bytes of x.  Scales (16 bits) and zero points (8 bits): per 16 rows
-// and group the pairs (row g, row g + 8), g = 0 .. 7.
+// Packed weights: a record per 128 rows (a slab; rows behind `hidden` are zeros) and 128 columns, slab by slab (the last record of
+// a slab holds 64 columns where K is not a multiple of 128):
+//   * per 64 columns [half of 32 columns][row][16 bytes], four words of eight columns; column c of eight is nibble c / 2 + 4 (c % 2), so
+//     that a word shifted by 4 i and masked is the pair of columns 2 i, 2 i + 1;
+//   * per group the slab's 128 scales of 16 bits, then, with zero points, per group 128 bytes.
 struct OprojInt4Params {
-  const uint16_t* x;          // [tokens, K], rows x_stride elements apart
-  int64_t x_stride;
-  const uint4* w;             // [hidden / 16][K / 64][32]
-  const uint32_t* scales;     // [hidden / 16][K / group][8]
-  const uint16_t* zeros;      // the same, or null
+  CUtensorMap x_map;          // [tokens, K], box (64, n_pad), SWIZZLE_128B
+  const uint8_t* w;           // packed, 16-byte aligned
   uint16_t* y;                // [tokens, hidden]
   int64_t y_stride;
-  int tokens, hidden, K, group, is_bf16;
+  int* error_flag;            // set to a helix::Status code when a bounded wait runs out
+  unsigned long long timeout_ns;
+  int tokens, hidden, K, group, zeros, is_bf16;
 };
 
-constexpr int kInt4MaxTokens = 16;       // of one launch
-constexpr int kInt4MaxK = 32768;
+constexpr int kInt4MaxTokens = 128;      // of one launch
+constexpr int int4_pad_tokens(int tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128; }
+constexpr size_t int4_slab_bytes(int64_t K, int64_t group, bool zeros) { return (size_t)(K * 64 + K / group * (zeros ? 384 : 256)); }
 cudaError_t launch_oproj_int4(const OprojInt4Params& p, bool pdl, int sm_count, cudaStream_t stream);
 
 }  // namespace helix

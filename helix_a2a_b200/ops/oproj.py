@@ -35,7 +35,9 @@ def oproj(x: torch.Tensor, w, *, splits: int = 0, library: Optional[bool] = None
     if isinstance(w, Int4OprojWeight):
         if not x.is_cuda:
             return (x.float() @ unpack_weight_int4(w).t()).to(x.dtype)
-        return _ext.ops().oproj_int4(x, w.packed, w.scales, w.zeros, w.hidden, w.K, w.group)
+        if x.dtype != w.dtype:
+            raise RuntimeError(f"x is {x.dtype}, the weight's scales are {w.dtype}")
+        return _ext.ops().oproj_int4(x, w.packed, w.hidden, w.K, w.group, w.zeros)
     if isinstance(w, PackedOprojWeight):
         if not x.is_cuda:
             return (x.float() @ unpack_weight(w).float().t()).to(x.dtype)
@@ -101,23 +103,32 @@ def unpack_weight(pw: PackedOprojWeight) -> torch.Tensor:
 
 class Int4OprojWeight:
     """A ``[hidden, K]`` weight in 4 bits with one scale (and zero point) per row and ``group`` columns: ``(q - z) * s`` with ``q`` and
-    ``z`` in 0 .. 15, ``z = 8`` where there are no zero points.  Laid out for the kernel (``csrc/oproj_int4.h``): per 16 rows and 64
-    columns the nibbles of every lane's matrix operands, scales and zero points as pairs of rows ``g`` and ``g + 8``.  Made by
-    :func:`quantize_weight_int4` from a matrix or by :func:`pack_weight_int4` from a checkpoint's arrays, once, at load time."""
+    ``z`` in 0 .. 15, ``z = 8`` where there are no zero points.  Laid out for the kernel (``csrc/oproj_int4.h``): a record per 128 rows
+    (those behind ``hidden`` are zeros) and 128 columns, its nibbles in the order in which they become matrix operands, then its scales and
+    zero points.  Made by :func:`quantize_weight_int4` from a matrix or by :func:`pack_weight_int4` from a checkpoint's arrays, once, at
+    load time."""
 
-    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], hidden: int, K: int, group: int):
-        self.packed, self.scales, self.zeros = packed, scales, zeros
-        self.hidden, self.K, self.group = hidden, K, group
+    def __init__(self, packed: torch.Tensor, hidden: int, K: int, group: int, dtype: torch.dtype, zeros: bool):
+        self.packed, self.hidden, self.K, self.group, self.dtype, self.zeros = packed, hidden, K, group, dtype, zeros
 
     @property
     def shape(self):
         return (self.hidden, self.K)
 
-
-def _row_pairs(t: torch.Tensor) -> torch.Tensor:
-    """``[hidden, groups]`` -> ``[hidden / 16, groups, 8, 2]``: rows ``g`` and ``g + 8`` of 16 side by side."""
-    hidden, groups = t.shape
-    return t.view(hidden // 16, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
+    def records(self):
+        """Views of the packed bytes, 128 columns at a time: nibbles ``[slabs, blocks of 64 columns, halves, 128 rows, 16 bytes]``, scales
+        ``[slabs, groups, 128]`` and zero points of that shape (or ``None``)."""
+        slabs, at = -(-self.hidden // 128), 0
+        rows = self.packed.view(slabs, -1)
+        for k in range(0, self.K, 128):
+            k1 = min(k + 128, self.K)
+            blocks, groups = (k1 - k) // 64, (k1 - k) // self.group
+            q, at = rows[:, at:at + blocks * 4096].unflatten(1, (blocks, 2, 128, 16)), at + blocks * 4096
+            s, at = rows[:, at:at + groups * 256].view(self.dtype).unflatten(1, (groups, 128)), at + groups * 256
+            z = None
+            if self.zeros:
+                z, at = rows[:, at:at + groups * 128].unflatten(1, (groups, 128)), at + groups * 128
+            yield slice(k, k1), q, s, z
 
 
 def pack_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None) -> Int4OprojWeight:
@@ -127,25 +138,37 @@ def pack_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zeros: Optiona
     group = K // max(scales.shape[-1], 1)
     if qweight.dtype != torch.uint8 or scales.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("pack_weight_int4 needs uint8 nibbles and bfloat16 or float16 scales")
-    if group not in (32, 64, 128) or scales.shape != (hidden, K // group) or hidden % 16 or K % 64 or K % group or not hidden or not K:
-        raise ValueError("pack_weight_int4 needs hidden % 16 == 0, K % 64 == 0 and scales [hidden, K / group], group 32, 64 or 128")
+    if group not in (32, 64, 128) or scales.shape != (hidden, K // group) or K % 64 or K % group or not hidden or not K:
+        raise ValueError("pack_weight_int4 needs K % 64 == 0 and scales [hidden, K / group], group 32, 64 or 128")
     if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
         raise ValueError("zeros must be uint8 of the scales' shape")
+    slabs = -(-hidden // 128)
+
+    def in_slabs(t):
+        t = torch.nn.functional.pad(t, (0, 0, 0, slabs * 128 - hidden)) if hidden % 128 else t
+        return t.view(slabs, 128, -1)
+
     q = torch.stack([qweight & 15, qweight >> 4], -1).view(hidden, K)
-    # row = 16 T + 8 r + g, column = 64 u + 32 c + 8 t + 4 o + 2 h + e (chunk, lane, step, half, element):
-    # word (c, o) of lane (g, t) has the nibble of register 2 h + r at 2 h + r, + 4 for the odd column
-    q = q.view(hidden // 16, 2, 8, K // 64, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)    # T u g t c o e h r
-    q = q.reshape(hidden // 16, K // 64, 32, 4, 4, 2)
-    packed = (q[..., 0] | (q[..., 1] << 4)).contiguous().view(-1)
-    return Int4OprojWeight(packed, _row_pairs(scales), None if zeros is None else _row_pairs(zeros), hidden, K, group)
+    # slab, row, block of 64, half, word, pair, column of the pair -> slab, block, half, row, word, nibble = pair + 4 * column
+    q = in_slabs(q).view(slabs, 128, K // 64, 2, 4, 4, 2).permute(0, 2, 3, 1, 4, 6, 5).reshape(slabs, K // 64, 2, 128, 16, 2)
+    q = q[..., 0] | (q[..., 1] << 4)
+    s, z = (None if t is None else in_slabs(t).transpose(1, 2) for t in (scales, zeros))
+    packed = torch.empty(slabs * (K * 64 + K // group * (256 if zeros is None else 384)), dtype=torch.uint8, device=qweight.device)
+    w = Int4OprojWeight(packed, hidden, K, group, scales.dtype, zeros is not None)
+    for cols, to_q, to_s, to_z in w.records():
+        to_q.copy_(q[:, cols.start // 64:cols.stop // 64])
+        to_s.copy_(s[:, cols.start // group:cols.stop // group])
+        if z is not None:
+            to_z.copy_(z[:, cols.start // group:cols.stop // group])
+    return w
 
 
 def quantize_weight_int4(w: torch.Tensor, group: int = 128, *, zero_points: bool = False) -> Int4OprojWeight:
     """Round a bf16 or fp16 ``[hidden, K]`` matrix to 4 bits, to the nearest: with zero points a group's range from its least to its
     largest value (and zero), without them -7 .. 7 times its largest magnitude / 7.  The scales have the matrix's type."""
     if w.dtype not in (torch.bfloat16, torch.float16) or w.dim() != 2 or group not in (32, 64, 128) or w.shape[1] % group or w.shape[1] % 64 \
-            or w.shape[0] % 16:
-        raise ValueError("quantize_weight_int4 needs a bfloat16 or float16 [hidden % 16 == 0, K % 64 == 0 and % group == 0] matrix")
+            or not w.numel():
+        raise ValueError("quantize_weight_int4 needs a bfloat16 or float16 [hidden, K % 64 == 0 and % group == 0] matrix")
     hidden, K = w.shape
     v = w.float().view(hidden, K // group, group)
     least = 2.0 ** -24                                   # a group of zeros has to have a scale, too
@@ -162,13 +185,13 @@ def quantize_weight_int4(w: torch.Tensor, group: int = 128, *, zero_points: bool
 
 def unpack_weight_int4(w: Int4OprojWeight) -> torch.Tensor:
     """The fp32 ``[hidden, K]`` matrix that a packed 4-bit weight stands for (oracles, debugging)."""
-    q = torch.stack([w.packed & 15, w.packed >> 4], -1).view(w.hidden // 16, w.K // 64, 8, 4, 2, 2, 2, 2, 2)   # T u g t c o e h r
-    q = q.permute(0, 8, 2, 1, 4, 3, 5, 7, 6).reshape(w.hidden, w.K // w.group, w.group).float()
-
-    def rows(t):
-        return t.permute(0, 3, 2, 1).reshape(w.hidden, -1, 1).float()
-
-    return ((q - (8.0 if w.zeros is None else rows(w.zeros))) * rows(w.scales)).view(w.hidden, w.K)
+    slabs = -(-w.hidden // 128)
+    out = torch.empty(slabs * 128, w.K, device=w.packed.device)
+    for cols, q, s, z in w.records():
+        q = torch.stack([q & 15, q >> 4], -1).view(slabs, -1, 2, 128, 4, 2, 4).permute(0, 3, 1, 2, 4, 6, 5)
+        q = q.reshape(slabs, 128, -1, w.group).float() - (8.0 if z is None else z.transpose(1, 2).unsqueeze(-1).float())
+        out[:, cols] = (q * s.transpose(1, 2).unsqueeze(-1).float()).view(slabs * 128, -1)
+    return out[:w.hidden]
 
 
 def check_compute_status(like: torch.Tensor) -> None:

@@ -14,7 +14,7 @@ def make(hidden, K, group, zeros, dtype, seed=0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     q = torch.randint(0, 16, (hidden, K), generator=g, dtype=torch.uint8, device="cuda")
     s = (torch.rand(hidden, K // group, generator=g, device="cuda") * 0.02 + 1e-3).to(dtype)
-    s[1] *= -1
+    s[1:2] *= -1
     z = torch.randint(0, 16, s.shape, generator=g, dtype=torch.uint8, device="cuda") if zeros else None
     w = oproj.pack_weight_int4(q[:, 0::2] | (q[:, 1::2] << 4), s, z)
     full = (q.double() - (8 if z is None else z.double().repeat_interleave(group, 1))) * s.double().repeat_interleave(group, 1)
@@ -34,15 +34,16 @@ def check(x, w, full):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("tokens", [1, 7, 8, 9, 16, 17, 33, 100])
+@pytest.mark.parametrize("tokens", [1, 7, 8, 9, 16, 17, 33, 64, 65, 100, 128, 129, 300])
 def test_types_groups_and_tokens(tokens, group, zeros, dtype):
     w, full = make(256, 1024, group, zeros, dtype)
     check(torch.randn(tokens, 1024, device="cuda").to(dtype), w, full)
 
 
-@pytest.mark.parametrize("tokens", [1, 5, 16, 40])
-@pytest.mark.parametrize("hidden,K,group", [(16, 64, 64), (16, 64, 32), (48, 192, 64), (4096, 832, 32), (144, 4160, 32), (2048, 2048, 128), (8192, 1024, 128),
-                                            (1024, 8192, 64), (32, 16384, 128), (48, 32768, 64), (20000, 320, 64), (7168, 4096, 128)])
+@pytest.mark.parametrize("tokens", [1, 16, 40, 100])
+@pytest.mark.parametrize("hidden,K,group", [(16, 64, 64), (16, 64, 32), (48, 192, 64), (1, 128, 128), (100, 256, 128), (130, 448, 64), (4096, 832, 32), (144, 4160, 32), (2048, 2048, 128), (8192, 1024, 128),
+                                            (1024, 8192, 64), (32, 16384, 128), (48, 32768, 64), (20000, 320, 64), (7168, 4096, 128), (7168, 16384, 64),
+                                            (9600, 32768, 32), (28672, 8192, 128)])
 def test_shapes(hidden, K, group, tokens):
     w, full = make(hidden, K, group, True, torch.bfloat16, seed=K)
     check(torch.randn(tokens, K, device="cuda").bfloat16(), w, full)
@@ -105,8 +106,9 @@ def test_no_tokens_and_refusals():
     for bad in (x.half(), x.float(), x[:, :128], x[0], odd[:, :256], torch.zeros(4, 257, dtype=torch.bfloat16, device="cuda")[:, :256], x.t()):
         with pytest.raises(RuntimeError):
             oproj.oproj(bad, w)
-    for key, bad in (("packed", w.packed[:-16]), ("scales", w.scales[:2].contiguous()), ("zeros", w.zeros.int()), ("scales", w.scales.half()), ("packed", w.packed.cpu())):
-        broken = oproj.Int4OprojWeight(w.packed, w.scales, w.zeros, w.hidden, w.K, w.group)
+    for key, bad in (("packed", w.packed[:-16]), ("packed", w.packed.cpu()), ("packed", w.packed.view(torch.int32)), ("zeros", False), ("group", 32),
+                     ("hidden", 160), ("group", 256), ("dtype", torch.float16), ("packed", torch.cat([w.packed[:1], w.packed])[1:])):
+        broken = oproj.Int4OprojWeight(w.packed, w.hidden, w.K, w.group, w.dtype, w.zeros)
         setattr(broken, key, bad)
         with pytest.raises(RuntimeError):
             oproj.oproj(x, broken)

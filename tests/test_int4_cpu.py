@@ -14,30 +14,31 @@ def arrays(hidden, K, group, zeros, dtype=torch.bfloat16, seed=0):
 
 
 @pytest.mark.parametrize("zeros", [False, True])
-@pytest.mark.parametrize("hidden,K,group", [(16, 64, 32), (16, 64, 64), (48, 192, 64), (32, 256, 128), (128, 832, 32)])
+@pytest.mark.parametrize("hidden,K,group", [(16, 64, 32), (16, 64, 64), (48, 192, 64), (32, 256, 128), (128, 832, 32), (300, 384, 128), (1, 64, 32)])
 def test_pack_and_unpack(hidden, K, group, zeros):
     q, s, z = arrays(hidden, K, group, zeros)
     w = oproj.pack_weight_int4(q[:, 0::2] | (q[:, 1::2] << 4), s, z)
-    assert w.shape == (hidden, K) and w.group == group and w.packed.numel() == hidden * K // 2
+    assert w.shape == (hidden, K) and w.group == group and w.packed.numel() == -(-hidden // 128) * 128 * (K // 2 + K // group * (3 if zeros else 2))
     want = (q.float() - (z.float() if zeros else torch.full(s.shape, 8.0)).repeat_interleave(group, 1)) * s.float().repeat_interleave(group, 1)
     assert torch.equal(oproj.unpack_weight_int4(w), want)
     x = torch.randn(3, K).bfloat16()
     assert torch.equal(oproj.oproj(x, w), (x.float() @ want.t()).bfloat16())
 
 
-def test_layout_of_one_lane():
+def test_layout():
     """The layout that csrc/oproj_int4.h states, nibble by nibble."""
-    q, s, _ = arrays(32, 128, 64, False)
-    w = oproj.pack_weight_int4(q[:, 0::2] | (q[:, 1::2] << 4), s)
-    words = w.packed.view(torch.int32).view(2, 2, 32, 4)
-    for tile, unit, lane, step in ((0, 0, 0, 0), (1, 1, 31, 3), (0, 1, 14, 2), (1, 0, 9, 1)):
-        g, t, word = lane >> 2, lane & 3, int(words[tile, unit, lane, step])
-        for i in range(8):
-            reg = i & 3
-            row = 16 * tile + g + 8 * (reg & 1)
-            col = 64 * unit + 32 * (step >> 1) + 8 * t + 4 * (step & 1) + 2 * (reg >> 1) + (i >> 2)
-            assert word >> (4 * i) & 15 == int(q[row, col])
-    assert torch.equal(w.scales[1, 1, 3], s[[16 + 3, 16 + 11], 1])
+    q, s, z = arrays(256, 192, 64, True)
+    w = oproj.pack_weight_int4(q[:, 0::2] | (q[:, 1::2] << 4), s, z)
+    slab = 192 * 64 + 3 * 384
+    for row, col in ((0, 0), (0, 1), (5, 31), (127, 32), (130, 63), (255, 64), (200, 127), (129, 128), (250, 191)):
+        rec, c = col // 128, col % 128
+        at = row // 128 * slab + rec * (128 * 64 + 2 * 384) + c // 64 * 4096 + c % 64 // 32 * 2048 + row % 128 * 16 + c % 32 // 8 * 4
+        word = int.from_bytes(bytes(w.packed[at:at + 4].tolist()), "little")
+        assert word >> (4 * (c % 8 // 2 + 4 * (c % 2))) & 15 == int(q[row, col])
+    scale_at = slab + 128 * 64 + 256                       # slab 1, record 0, group 1
+    assert torch.equal(w.packed[scale_at:scale_at + 256].view(torch.bfloat16), s[128:, 1])
+    zero_at = slab + 128 * 64 + 2 * 384 + 64 * 64 + 256    # slab 1, record 1, group 2
+    assert torch.equal(w.packed[zero_at:zero_at + 128], z[128:, 2])
 
 
 @pytest.mark.parametrize("zero_points", [False, True])
@@ -47,7 +48,7 @@ def test_quantisation_is_off_by_half_a_step(dtype, zero_points):
     w[3] = 0
     w[4, :64] = 0.5
     pw = oproj.quantize_weight_int4(w, 64, zero_points=zero_points)
-    step = pw.scales.permute(0, 3, 2, 1).reshape(64, -1).float().repeat_interleave(64, 1)
+    step = torch.cat([sc[0, :, :64].t() for _, _, sc, _ in pw.records()], 1).float().repeat_interleave(64, 1)
     # half a step for the rounding; the scale and the zero point are rounded too, which the ends of the range feel (up to 7.5 steps
     # eps / 2 each, and with zero points another half step where the range is clamped)
     tol = step * (0.5 + 8 * torch.finfo(dtype).eps + (0.5 if zero_points else 0))
@@ -58,12 +59,12 @@ def test_quantisation_is_off_by_half_a_step(dtype, zero_points):
 def test_refusals():
     q, s, z = arrays(32, 128, 64, True)
     b = q[:, 0::2] | (q[:, 1::2] << 4)
-    for bad in ((b.int(), s, z), (b, s.float(), z), (b, s[:, :1].repeat(1, 3), z), (b[:24], s[:24], z[:24]), (b, s, z[:16]), (b, s, z.int()),
+    for bad in ((b.int(), s, z), (b, s.float(), z), (b, s[:, :1].repeat(1, 3), z), (b, s, z[:16]), (b, s, z.int()),
                 (b[:, :16], s, z), (b[:0], s[:0], None)):
         with pytest.raises(ValueError):
             oproj.pack_weight_int4(*bad)
     w = torch.zeros(32, 128, dtype=torch.bfloat16)
-    for bad in (w.float(), w[:24], w[:, :96]):
+    for bad in (w.float(), w[:0], w[:, :96], w[0]):
         with pytest.raises(ValueError):
             oproj.quantize_weight_int4(bad, 64)
     with pytest.raises(ValueError):
