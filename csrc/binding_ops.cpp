@@ -557,14 +557,16 @@ torch::Tensor oproj_int4(torch::Tensor x, torch::Tensor packed, int64_t hidden, 
   torch::Tensor y = torch::empty({tokens, hidden}, x.options());
   if (tokens == 0) return y;
   ScratchUse sc = scratch_for(dev, false, 0, 0, 0);
-  for (int64_t t0 = 0; t0 < tokens; t0 += helix::kInt4MaxTokens) {
+  for (int64_t t0 = 0; t0 < tokens; t0 += helix::int4_max_tokens((int)group)) {
     helix::OprojInt4Params p{};
-    p.tokens = (int)std::min<int64_t>(tokens - t0, helix::kInt4MaxTokens);
+    p.tokens = (int)std::min<int64_t>(tokens - t0, helix::int4_max_tokens((int)group));
+    p.x = reinterpret_cast<const uint16_t*>(x.data_ptr()) + t0 * x.stride(0);
+    p.x_stride = x.stride(0);
     const uint64_t dims[2] = {(uint64_t)K, (uint64_t)p.tokens}, strides[1] = {(uint64_t)(p.tokens > 1 ? x.stride(0) : K) * 2};
     const uint32_t box[2] = {64, (uint32_t)helix::int4_pad_tokens(p.tokens)};
     const char* err = nullptr;
     TORCH_CHECK(helix::encode_tensor_map(&p.x_map, type == at::ScalarType::Half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                                         reinterpret_cast<uint16_t*>(x.data_ptr()) + t0 * x.stride(0), dims, strides, box, helix::TmaSwizzle::k128B, &err),
+                                         p.x, dims, strides, box, helix::TmaSwizzle::k128B, &err),
                 "helix: activation tensor map: ", err ? err : "?");
     p.w = packed.data_ptr<uint8_t>();
     p.y = reinterpret_cast<uint16_t*>(y.data_ptr()) + t0 * hidden;

@@ -116,18 +116,18 @@ class Int4OprojWeight:
         return (self.hidden, self.K)
 
     def records(self):
-        """Views of the packed bytes, 128 columns at a time: nibbles ``[slabs, blocks of 64 columns, halves, 128 rows, 16 bytes]``, scales
-        ``[slabs, groups, 128]`` and zero points of that shape (or ``None``)."""
+        """Views of the packed bytes, 128 columns at a time: nibbles ``[slabs, 8 tiles, blocks of 32 columns, 16 rows, 16 bytes]``, scales
+        ``[slabs, groups, 8 tiles, 8, 2]`` and zero points of that shape (or ``None``)."""
         slabs, at = -(-self.hidden // 128), 0
         rows = self.packed.view(slabs, -1)
         for k in range(0, self.K, 128):
             k1 = min(k + 128, self.K)
-            blocks, groups = (k1 - k) // 64, (k1 - k) // self.group
-            q, at = rows[:, at:at + blocks * 4096].unflatten(1, (blocks, 2, 128, 16)), at + blocks * 4096
-            s, at = rows[:, at:at + groups * 256].view(self.dtype).unflatten(1, (groups, 128)), at + groups * 256
+            blocks, groups = (k1 - k) // 32, (k1 - k) // self.group
+            q, at = rows[:, at:at + blocks * 2048].unflatten(1, (8, blocks, 16, 16)), at + blocks * 2048
+            s, at = rows[:, at:at + groups * 256].view(self.dtype).unflatten(1, (groups, 8, 8, 2)), at + groups * 256
             z = None
             if self.zeros:
-                z, at = rows[:, at:at + groups * 128].unflatten(1, (groups, 128)), at + groups * 128
+                z, at = rows[:, at:at + groups * 128].unflatten(1, (groups, 8, 8, 2)), at + groups * 128
             yield slice(k, k1), q, s, z
 
 
@@ -149,14 +149,15 @@ def pack_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zeros: Optiona
         return t.view(slabs, 128, -1)
 
     q = torch.stack([qweight & 15, qweight >> 4], -1).view(hidden, K)
-    # slab, row, block of 64, half, word, pair, column of the pair -> slab, block, half, row, word, nibble = pair + 4 * column
-    q = in_slabs(q).view(slabs, 128, K // 64, 2, 4, 4, 2).permute(0, 2, 3, 1, 4, 6, 5).reshape(slabs, K // 64, 2, 128, 16, 2)
+    # slab, tile, row, block of 32, word, pair, column of the pair -> slab, tile, block, row, word, nibble = pair + 4 * column
+    q = in_slabs(q).view(slabs, 8, 16, K // 32, 4, 4, 2).permute(0, 1, 3, 2, 4, 6, 5).reshape(slabs, 8, K // 32, 16, 16, 2)
     q = q[..., 0] | (q[..., 1] << 4)
-    s, z = (None if t is None else in_slabs(t).transpose(1, 2) for t in (scales, zeros))
+    # slab, tile, upper or lower eight rows, row, group -> slab, group, tile, row, half
+    s, z = (None if t is None else in_slabs(t).view(slabs, 8, 2, 8, K // group).permute(0, 4, 1, 3, 2) for t in (scales, zeros))
     packed = torch.empty(slabs * (K * 64 + K // group * (256 if zeros is None else 384)), dtype=torch.uint8, device=qweight.device)
     w = Int4OprojWeight(packed, hidden, K, group, scales.dtype, zeros is not None)
     for cols, to_q, to_s, to_z in w.records():
-        to_q.copy_(q[:, cols.start // 64:cols.stop // 64])
+        to_q.copy_(q[:, :, cols.start // 32:cols.stop // 32])
         to_s.copy_(s[:, cols.start // group:cols.stop // group])
         if z is not None:
             to_z.copy_(z[:, cols.start // group:cols.stop // group])
@@ -188,9 +189,12 @@ def unpack_weight_int4(w: Int4OprojWeight) -> torch.Tensor:
     slabs = -(-w.hidden // 128)
     out = torch.empty(slabs * 128, w.K, device=w.packed.device)
     for cols, q, s, z in w.records():
-        q = torch.stack([q & 15, q >> 4], -1).view(slabs, -1, 2, 128, 4, 2, 4).permute(0, 3, 1, 2, 4, 6, 5)
-        q = q.reshape(slabs, 128, -1, w.group).float() - (8.0 if z is None else z.transpose(1, 2).unsqueeze(-1).float())
-        out[:, cols] = (q * s.transpose(1, 2).unsqueeze(-1).float()).view(slabs * 128, -1)
+        q = torch.stack([q & 15, q >> 4], -1).view(slabs, 8, -1, 16, 4, 2, 4).permute(0, 1, 3, 2, 4, 6, 5).reshape(slabs * 128, -1, w.group)
+
+        def rows(t):
+            return t.permute(0, 2, 4, 3, 1).reshape(slabs * 128, -1, 1).float()
+
+        out[:, cols] = ((q.float() - (8.0 if z is None else rows(z))) * rows(s)).flatten(1)
     return out[:w.hidden]
 
 

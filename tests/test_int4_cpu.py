@@ -32,13 +32,14 @@ def test_layout():
     slab = 192 * 64 + 3 * 384
     for row, col in ((0, 0), (0, 1), (5, 31), (127, 32), (130, 63), (255, 64), (200, 127), (129, 128), (250, 191)):
         rec, c = col // 128, col % 128
-        at = row // 128 * slab + rec * (128 * 64 + 2 * 384) + c // 64 * 4096 + c % 64 // 32 * 2048 + row % 128 * 16 + c % 32 // 8 * 4
+        at = row // 128 * slab + rec * (128 * 64 + 2 * 384) + row % 128 // 16 * (256 if rec else 512) * 2 + c // 32 * 256 + row % 16 * 16 + c % 32 // 8 * 4
         word = int.from_bytes(bytes(w.packed[at:at + 4].tolist()), "little")
         assert word >> (4 * (c % 8 // 2 + 4 * (c % 2))) & 15 == int(q[row, col])
     scale_at = slab + 128 * 64 + 256                       # slab 1, record 0, group 1
-    assert torch.equal(w.packed[scale_at:scale_at + 256].view(torch.bfloat16), s[128:, 1])
+    order = [16 * tile + g + 8 * half for tile in range(8) for g in range(8) for half in range(2)]
+    assert torch.equal(w.packed[scale_at:scale_at + 256].view(torch.bfloat16), s[128:, 1][order])
     zero_at = slab + 128 * 64 + 2 * 384 + 64 * 64 + 256    # slab 1, record 1, group 2
-    assert torch.equal(w.packed[zero_at:zero_at + 128], z[128:, 2])
+    assert torch.equal(w.packed[zero_at:zero_at + 128], z[128:, 2][order])
 
 
 @pytest.mark.parametrize("zero_points", [False, True])
@@ -48,7 +49,7 @@ def test_quantisation_is_off_by_half_a_step(dtype, zero_points):
     w[3] = 0
     w[4, :64] = 0.5
     pw = oproj.quantize_weight_int4(w, 64, zero_points=zero_points)
-    step = torch.cat([sc[0, :, :64].t() for _, _, sc, _ in pw.records()], 1).float().repeat_interleave(64, 1)
+    step = torch.cat([sc[0, :, :4].permute(1, 3, 2, 0).reshape(64, -1) for _, _, sc, _ in pw.records()], 1).float().repeat_interleave(64, 1)
     # half a step for the rounding; the scale and the zero point are rounded too, which the ends of the range feel (up to 7.5 steps
     # eps / 2 each, and with zero points another half step where the range is clamped)
     tol = step * (0.5 + 8 * torch.finfo(dtype).eps + (0.5 if zero_points else 0))
