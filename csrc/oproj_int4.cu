@@ -9,10 +9,11 @@
 // holds as B operands for the whole launch, and walks over 16-row tiles, the next tile's weights on their way.
 //
 // More tokens (oproj_int4_kernel) run on tcgen05.  A CTA owns a slab of 128 rows (M of the MMA; tokens are N) and a run of columns.
-//   * Records of the packed weight arrive by bulk copy.  Eight warps turn nibbles into numbers and put them into tensor memory as the
-//     MMA's A operand, a thread per row and 64 columns.  (In shared memory a record is 32 KB written and 32 KB read for 8 KB that arrived.)
-//   * Every group has an accumulator of its own in tensor memory, filled while the next record is turned into numbers; then the same warps, a
-//     thread per row and half of the tokens, add it, times its scale, to their sums in registers.
+//   * Records of the packed weight arrive by bulk copy.  Two teams of eight warps take them in turn, turn nibbles into numbers and put them
+//     into tensor memory as the MMA's A operand, a thread per row and 64 columns.  (In shared memory a record is 32 KB written and 32 KB read
+//     for 8 KB that arrived.  A record is a chain of waits, loads and stores of ~1600 cycles for its team, so one team alone is half as fast.)
+//   * Every group of a record has an accumulator of its own in tensor memory, filled while the team turns its next record into numbers;
+//     then the same warps, a thread per row and half of the tokens, add it, times its scale, to their sums in registers.
 //   * One barrier tells the MMA warp that a record is in place, its x too, and the accumulators read; one that its MMAs are through.
 //
 // In both the warps or CTAs that share out the columns meet in shared memory, across a cluster by distributed shared memory: no scratch
@@ -37,8 +38,7 @@ namespace {
 using namespace sm100;
 
 constexpr int kRows = 128;
-constexpr int kWorkers = 8, kParts = kWorkers / 4;     // warps that dequantise; threads that share a row
-constexpr int kMmaWarp = kWorkers, kThreads = (kWorkers + 2) * 32;               // and a warp that loads
+constexpr int kTeam = 8, kParts = kTeam / 4;     // warps that dequantise; threads that share a row
 constexpr int kOperand = 64;                           // columns of tensor memory of a record's A operand
 constexpr int kNibbles = 4096;                         // packed bytes of 64 columns
 constexpr int kMaxRecord = 2 * kNibbles + 4 * 384;     // 128 columns in groups of 32, with zero points
@@ -49,16 +49,19 @@ constexpr int kFewSmem = 200 * 1024;
 
 template <int N>
 struct Shape {
-  static constexpr int ctas = N <= 32 ? 2 : 1;         // per SM
-  static constexpr int slots = 2;                      // records between dequantisation and MMA
+  // With more than 64 tokens the sums take the registers of a second team, and its accumulators the tensor memory.
+  static constexpr int teams = N <= 64 ? 2 : 1, workers = teams * kTeam;
+  static constexpr int mma_warp = workers, threads = (workers + 2) * 32;           // and a warp that loads
+  static constexpr int slots = 2 * teams;              // records between dequantisation and MMA
   static constexpr int stages = 8;                     // packed records on their way
-  static constexpr int accs = N <= 64 ? 4 : 2;         // groups of a record: with more than 64 tokens none of 32 columns
-  static constexpr int a_col = accs * N;               // tensor memory: accumulators, then operands
-  static constexpr int cols = a_col + slots * kOperand <= 256 ? 256 : 512;
+  static constexpr int accs = N <= 32 ? 4 : 2;     // groups of a record: more tokens want larger groups (int4_max_tokens)
+  static constexpr int a_col = teams * accs * N;      // tensor memory: accumulators, then operands
+  static_assert(a_col + slots * kOperand <= 512);
   static constexpr int x_bytes = N * 128;              // B operand of 64 columns
   static constexpr int ring = slots * 2 * x_bytes + stages * kMaxRecord;
-  static constexpr int row = N * 4 + 16;               // bytes between rows of sums that CTAs send each other, up to 168 rows
-  static constexpr int smem = (ring > 168 * row ? ring : 168 * row) + 1024;
+  static constexpr int row = N * 4 + 16;               // bytes between rows of sums on their way, up to 168 rows of either team
+  static constexpr int sums = teams * 168 * row;
+  static constexpr int smem = (ring > sums ? ring : sums) + 1024;
 };
 
 template <bool BF16>
@@ -95,7 +98,7 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[N]) {
 }
 
 template <bool BF16, int N>
-__global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(const __grid_constant__ OprojInt4Params p) {
+__global__ void __launch_bounds__(Shape<N>::threads, 1) oproj_int4_kernel(const __grid_constant__ OprojInt4Params p) {
   using S = Shape<N>;
   constexpr int NT = N / kParts;                       // tokens of a worker thread
   extern __shared__ uint8_t smem_raw[];
@@ -113,17 +116,17 @@ __global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(co
   if (tid == 0) {
     for (int i = 0; i < S::stages; ++i) {
       mbar_init(&w_full[i], 1);
-      mbar_init(&w_free[i], kWorkers);
+      mbar_init(&w_free[i], kTeam);
     }
     for (int i = 0; i < S::slots; ++i) {
-      mbar_init(&a_full[i], kWorkers + 1);             // and the bytes of x
+      mbar_init(&a_full[i], kTeam + 1);                // and the bytes of x
       mbar_init(&a_free[i], 1);
     }
     mbar_init(&drain, 1);
     mbar_fence_init();
   }
-  if (warp == kMmaWarp) {
-    tmem_alloc(&tmem_slot, S::cols);
+  if (warp == S::mma_warp) {
+    tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -136,25 +139,25 @@ __global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(co
   float acc[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j] = 0.f;
-  if (warp < kWorkers) {
+  if (warp < S::workers) {
     // =========================== dequantisation, and the sums ===========================
-    const int row = tid & (kRows - 1), part = tid >> 7;              // 64 of a record's columns; half of the tokens
+    const int row = tid & (kRows - 1), part = tid >> 7 & 1, team = tid >> 8;               // 64 of a record's columns; half of the tokens
     const int pair = (row & ~15) + (row & 7) * 2 + (row >> 3 & 1);   // of the row among the scales
-    const uint32_t tq = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + part * NT;
+    const uint32_t tq = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + team * (S::accs * N) + part * NT;
     // both in registers: with two constants the compiler makes two instructions of (w & mask) | magic
     uint32_t mask, magic;
     asm volatile("mov.u32 %0, 0x000f000f;" : "=r"(mask));
     asm volatile("mov.u32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300 : 0x64006400));
     // x of record r, into the place that record r - slots has left
     auto load_x = [&](int r) {
-      if (warp != 0 || lane != 0 || r >= records) return;
+      if (warp % kTeam != 0 || lane != 0 || r >= records) return;
       const int sl = r % S::slots, cols = columns(r);
       mbar_expect_tx(&a_full[sl], cols / 64 * S::x_bytes);
       for (int c = 0; c < cols; c += 64)
         tma_load_2d(x_ring + (sl * 2 + c / 64) * S::x_bytes, &p.x_map, &a_full[sl], (r0 + r) * 128 + c, 0);
     };
-    if (warp == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int r = 0; r < S::slots; ++r) load_x(r);
+    if (warp % kTeam == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int r = team; r < S::slots; r += S::teams) load_x(r);
     float s[S::accs], s_last[S::accs];                             // scales of the row's groups, of this record and of the one before
     int groups = 0;
     // the groups of record r, whose MMAs are waited for
@@ -178,7 +181,8 @@ __global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(co
       }
       tc_fence_before_sync();
     };
-    for (int r = 0; r < records; ++r) {
+    int last = -1;                                     // the team's record before
+    for (int r = team; r < records; last = r, r += S::teams) {
       const int st = r % S::stages, sl = r % S::slots, cols = columns(r);
       ok = __all_sync(0xffffffffu, mbar_wait(&w_full[st], (r / S::stages) & 1, deadline));
       if (!ok) break;
@@ -207,9 +211,9 @@ __global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(co
         tmem_st_wait();
         tc_fence_before_sync();
       }
-      if (r > 0) {
-        add_groups(r - 1);
-        if (ok) load_x(r + S::slots - 1);
+      if (last >= 0) {
+        add_groups(last);
+        if (ok) load_x(last + S::slots);
       }
       groups = cols >> gshift;
       __syncwarp();
@@ -221,8 +225,8 @@ __global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(co
     }
 #pragma unroll
     for (int i = 0; i < S::accs; ++i) s_last[i] = s[i];
-    if (ok) add_groups(records - 1);
-  } else if (warp == kMmaWarp) {
+    if (ok && last >= 0) add_groups(last);
+  } else if (warp == S::mma_warp) {
     // =========================== MMA issue ===========================
     constexpr uint32_t idesc = BF16 ? umma_idesc_bf16(kRows, N) : umma_idesc_bf16(kRows, N) & ~((1u << 7) | (1u << 10));
     const uint64_t d_x = umma_desc_k_sw128(smem_u32(x_ring));
@@ -234,12 +238,12 @@ __global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(co
         ok = __all_sync(0xffffffffu, mbar_wait(&a_full[sl], (r / S::slots) & 1, deadline));
         if (!ok) break;
         tc_fence_after_sync();
-        const uint32_t ta = tmem + S::a_col + sl * kOperand, x_lo = (uint32_t)d_x + (sl * 2 * S::x_bytes >> 4), x_hi = (uint32_t)(d_x >> 32);
+        const uint32_t td = tmem + r % S::teams * (S::accs * N), ta = tmem + S::a_col + sl * kOperand, x_lo = (uint32_t)d_x + (sl * 2 * S::x_bytes >> 4), x_hi = (uint32_t)(d_x >> 32);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 128; k += 16) {
             if (k == 64 && cols == 64) break;
-            const uint32_t lo = x_lo + ((k / 64 * S::x_bytes + k % 64 * 2) >> 4), d = tmem + (k >> kShift) * N;
+            const uint32_t lo = x_lo + ((k / 64 * S::x_bytes + k % 64 * 2) >> 4), d = td + (k >> kShift) * N;
             if (k % (1 << kShift) == 0) umma_bf16_ts_first(d, ta + k / 2, lo, x_hi, idesc, 0u);
             else umma_bf16_ts(d, ta + k / 2, lo, x_hi, idesc);
           }
@@ -284,44 +288,42 @@ __global__ void __launch_bounds__(kThreads, Shape<N>::ctas) oproj_int4_kernel(co
     while (now_ns() < limit) {
     }
   }
-  if (warp == kMmaWarp) {
+  if (warp == S::mma_warp) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, S::cols);
+    tmem_dealloc(tmem, 512);
   }
 
-  // ---- results: thread (row, part) holds tokens part * NT ... of its row ----------------------------------
-  const int row = tid & (kRows - 1), part = tid >> 7;
-  const int rows_here = min(kRows, p.hidden - slab * kRows);
-  if (cl == 1) {
-    if (warp < kWorkers && row < rows_here) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int n = part * NT + j;
-        if (n < p.tokens) p.y[n * p.y_stride + slab * kRows + row] = narrow<BF16>(acc[j]);
-      }
-    }
-    return;
-  }
-  // Rank r finishes rows r * per ... of the slab.  Everybody is through with its rings, so they take the others' sums.
+  // ---- results: thread (team, part, row) holds tokens part * NT ... of its row, the sum over its team's records ------
+  // Rank r finishes rows r * per ... of the slab.  Everybody is through with its rings, so they take the sums: [rank][team][row].
+  const int row = tid & (kRows - 1), part = tid >> 7 & 1, team = tid >> 8, rows_here = min(kRows, p.hidden - slab * kRows);
   const int per = (kRows / 8 + cl - 1) / cl * 8;
-  __syncwarp();
-  cluster_arrive();
-  cluster_wait();
-  if (warp < kWorkers) {
-    const uint32_t to = map_to_cta(smem_u32(smem) + (rank * per + row % per) * S::row + part * NT * 4, row / per);
+  auto meet = [&]() {
+    if (cl == 1) {
+      __syncthreads();
+    } else {
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+    }
+  };
+  meet();
+  if (warp < S::workers) {
+    const uint32_t at = smem_u32(smem) + ((rank * S::teams + team) * per + row % per) * S::row + part * NT * 4;
+    const uint32_t to = cl == 1 ? at : map_to_cta(at, row / per);
 #pragma unroll
-    for (int j = 0; j < NT; j += 4) st_cluster_f32x4(to + j * 4, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+    for (int j = 0; j < NT; j += 4) {
+      if (cl == 1) *reinterpret_cast<float4*>(smem + (at - smem_u32(smem)) + j * 4) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+      else st_cluster_f32x4(to + j * 4, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+    }
   }
-  __syncwarp();
-  cluster_arrive();
-  cluster_wait();
+  meet();
   const int mine = max(min(per, rows_here - rank * per), 0);
-  for (int e = tid; e < per * p.tokens; e += kThreads) {
+  for (int e = tid; e < per * p.tokens; e += S::threads) {
     const int n = e / per, r = e % per;
     if (r >= mine) continue;
     const uint8_t* from = smem + r * S::row + n * 4;
     float v = *reinterpret_cast<const float*>(from);
-    for (int c = 1; c < cl; ++c) v += *reinterpret_cast<const float*>(from + c * per * S::row);
+    for (int c = 1; c < cl * S::teams; ++c) v += *reinterpret_cast<const float*>(from + c * per * S::row);
     p.y[n * p.y_stride + slab * kRows + rank * per + r] = narrow<BF16>(v);
   }
 }
@@ -413,8 +415,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) oproj_int4_few_kernel(const
     const int batch = min(p.batch, all - j0);
 #pragma unroll 1
     for (int j = j0; j < j0 + batch; ++j) {
+      // with two tiles of tokens the registers do not hold a second tile of weights (8192 x 8192: 23.1 us with it, spilled, 16.6 without)
+      if (NT == 2 && j > 0) fetch(blockIdx.x + j * step, next);
       const Tile f = next;
-      fetch(blockIdx.x + (j + 1) * step, next);
+      if (NT == 1) fetch(blockIdx.x + (j + 1) * step, next);
       float acc[NT][4], part[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -516,10 +520,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) oproj_int4_few_kernel(const
 
 using Fn = void (*)(OprojInt4Params);
 template <bool BF16>
-Fn pick(int n, size_t* smem) {
-  if (n == 32) return *smem = Shape<32>::smem, (Fn)oproj_int4_kernel<BF16, 32>;
-  if (n == 64) return *smem = Shape<64>::smem, (Fn)oproj_int4_kernel<BF16, 64>;
-  return *smem = Shape<128>::smem, (Fn)oproj_int4_kernel<BF16, 128>;
+Fn pick(int n, int* threads, size_t* smem) {
+  if (n == 32) return *threads = Shape<32>::threads, *smem = Shape<32>::smem, (Fn)oproj_int4_kernel<BF16, 32>;
+  if (n == 64) return *threads = Shape<64>::threads, *smem = Shape<64>::smem, (Fn)oproj_int4_kernel<BF16, 64>;
+  return *threads = Shape<128>::threads, *smem = Shape<128>::smem, (Fn)oproj_int4_kernel<BF16, 128>;
 }
 template <bool BF16, int NT>
 Fn pick_few(int group, bool zeros) {
@@ -606,14 +610,15 @@ cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStr
     return cudaErrorInvalidValue;
   int dev = 0;
   cudaGetDevice(&dev);
-  // Few tokens: 8192 x 8192, 8 tokens FEW_US us against BIG_US, 16 tokens FEW16_US against BIG16_US.  A wider K than a cluster's warps hold
-  // takes the other kernel.
+  // Measured in graphs, 8192 x 8192: 8 tokens 12.1 us, 16 tokens 16.6 (two launches of eight 24), the other kernel 24.2 from 17 tokens on.  A
+  // wider K than a cluster's warps hold takes the other kernel, too.
   if (p.tokens <= kInt4FewTokens && p.K <= kMaxCluster * kFewWarps * 256) return launch_few(p, pdl, sm_count, dev, stream);
   size_t smem = 0;
   const int n = int4_pad_tokens(p.tokens);
-  const Fn fn = p.is_bf16 ? pick<true>(n, &smem) : pick<false>(n, &smem);
+  int threads = 0;
+  const Fn fn = p.is_bf16 ? pick<true>(n, &threads, &smem) : pick<false>(n, &threads, &smem);
   Resident r;
-  const cudaError_t e = resident((const void*)fn, dev, kThreads, smem, smem, sm_count, &r);
+  const cudaError_t e = resident((const void*)fn, dev, threads, smem, smem, sm_count, &r);
   if (e != cudaSuccess) return e;
   // As many CTAs per slab as make the launch shortest: rounds of resident clusters times the records of a CTA, and about three records'
   // time for a CTA's start, the exchange and the end.
@@ -629,7 +634,7 @@ cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStr
     }
   }
   cudaLaunchAttribute attrs[2];
-  const cudaLaunchConfig_t cfg = config(slabs, best, kThreads, smem, pdl, stream, attrs);
+  const cudaLaunchConfig_t cfg = config(slabs, best, threads, smem, pdl, stream, attrs);
   return cudaLaunchKernelEx(&cfg, fn, p);
 }
 
