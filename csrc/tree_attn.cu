@@ -7,9 +7,11 @@
 //
 // A group of 8 heads and 16 drafted tokens fill the 128 rows of one tensor-core tile, so both products run on tcgen05: S = Q K^T with
 // both operands in shared memory, P back into tensor memory over S, O += P V with V as it lies in the cache (MN-major).
-//   * Two streams per CTA keep the tensor cores busy: while one softmax warpgroup (a thread per row) works on its scores, the
-//     other stream's products run.  With more than 128 rows (`tiles` = 2) a stream is a tile of rows and every KV tile serves both;
-//     with up to 128 rows the streams take alternate KV tiles of the same rows, and their sums are joined at the end.
+//   * Two streams per CTA, a softmax warpgroup each (a thread per row), keep tensor cores and exponentials busy.  With more than 128 rows
+//     (`tiles` = 2) a stream is a tile of rows and every KV tile serves both.  With up to 128 rows a stream is half of every KV tile's
+//     tokens, for all rows, with sums of its own that are joined at the end; scores have two buffers then, so that the next tile's are
+//     there when this one's probabilities are.  (Streams that took alternate KV tiles held two tiles' V each through their softmax, which
+//     left one place of the ring for loads: 128k tokens, 16 drafted 141 us.)
 //   * The KV tiles of all (sequence, row tile, KV head) units form one line that is cut into equal shares, a CTA per SM.  A unit that
 //     does not lie inside one share is left in pieces (normalised rows and their LSE), which a second kernel folds.
 //   * The mask only concerns tiles that reach behind the committed tokens: there a row's mask words are shifted into place.
@@ -174,11 +176,10 @@ __device__ __forceinline__ uint32_t mask_bits(const uint64_t* words, int n_words
 template <bool BF16, int MT>
 __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_constant__ TreeDecodeParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t kv_full[kSlots], kv_free[kSlots], s_full[2], p_full[2][2], o_full[2], q_full, idle, scrubbed, turn[2], drain[2];
+  __shared__ __align__(8) uint64_t kv_full[kSlots], kv_free[kSlots], s_full[2], p_full[2][2], o_full[2], q_full, scrubbed, turn[2], drain[2];
   __shared__ uint32_t tmem_slot, s_poison[2][2 * kTreeMaxWords];      // by turns: a segment's is cleared behind its end
   __shared__ float s_x[2][kRows];                  // what the streams tell each other at the end of a segment
   __shared__ int s_rest;
-  __shared__ uint32_t s_issued;                    // tiles (K and V apart) whose loads have been started
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + 2 * kSlotBytes;           // behind two tiles of Q: both row tiles, or this segment's and the next one's
@@ -193,18 +194,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i][0], 4);                 // halves of 64 tokens
+      mbar_init(&p_full[i][0], 4);                 // halves of 64 tokens; with one row tile, every other KV tile
       mbar_init(&p_full[i][1], 4);
       mbar_init(&turn[i], 4);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(&q_full, kSmWarps);
-    mbar_init(&idle, 1);
     mbar_init(&scrubbed, kSmWarps);
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     s_rest = 0;
-    s_issued = 0;
     mbar_fence_init();
   }
   if (tid < 4 * kTreeMaxWords) s_poison[0][tid] = 0;
@@ -279,18 +278,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
   bool ok = true;
   uint32_t gt = 0;                                 // KV tiles this CTA has been through: fixes slots and phases
 
-  // The wait for entry r of the ring.  Loads complete in any order, and with one row tile a stream only sees every other tile: entry
-  // r - kSlots may have been the other stream's and still be on its way, and then the parity of r would be taken for the one before.  The
-  // loader starts an entry when its place has been read to the end, so from then on the parity means r.
-  auto tile_there = [&](uint32_t r) {
-    if (MT == 1) {
-      unsigned spins = 0;
-      while (*reinterpret_cast<volatile uint32_t*>(&s_issued) <= r)
-        if ((++spins & 255u) == 0u && now_ns() > deadline) return false;
-    }
-    return mbar_wait(&kv_full[r % kSlots], (r / kSlots) & 1, deadline);
-  };
-
   if (warp < kSmWarps) {
     // =========================== softmax ===========================
     // 2 * 216 + 72 registers per thread of a warpgroup are what the block was launched with, 3 * 168
@@ -298,12 +285,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     const int st = warp >> 2;                      // this warpgroup's stream
     const int quad = warp & 3, row = 32 * quad + lane;
     const uint32_t tq = tmem + ((uint32_t)(32 * quad) << 16);
-    const uint32_t col_s = kColS + 128 * st, col_o = kColO + 128 * st;
+    const uint32_t col_o = kColO + 128 * st;
+    constexpr int kHere = MT == 1 ? 64 : 128, kChunks = kHere / 32;  // tokens of a tile that this stream takes
+    const int first = MT == 1 ? 64 * st : 0;
     constexpr float kBias = BF16 ? 0.f : 7.f;
     const float sl2 = p.scale * kLog2e;
     const float2 sl22 = make_float2(sl2, sl2);
     uint32_t steps = 0, n_seg = 0, n_scrub = 0;    // of this stream, over all segments
-    uint32_t n_joined = 0, n_idle = 0;             // one row tile: segments in which both streams had a part, and the others
 
     // Q of a segment into shared memory: K-major, 128-byte swizzle, halves of 64 dims
     auto load_q = [&](const Segment& sg, uint32_t n) {
@@ -332,24 +320,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       const uint64_t* words = p.mask + (valid ? qrow : 0) * p.mask_stride;
       float m = -INFINITY, l = 0.f;
       bool huge = false;
-      const int n_steps = MT == 2 ? seg.count : (seg.count - st + 1) / 2;
 
-      for (int k = 0; k < n_steps; ++k, ++steps) {
-        const int i = MT == 2 ? k : 2 * k + st;                      // tile of the segment
+      for (int i = 0; i < seg.count; ++i, ++steps) {
         const int tok0 = (seg.t_begin + i) * kTile;
         const bool special = tok0 + kTile > committed;               // reaches behind the committed tokens
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[st], steps & 1, deadline));
+        // the scores' place: the stream's own, or the tile's
+        const int buf = MT == 1 ? steps & 1 : st;
+        const uint32_t col_s = kColS + 128 * buf + first;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buf], (MT == 1 ? steps >> 1 : steps) & 1, deadline));
         if (!ok) break;
         tc_fence_after_sync();
         if (special) {
           // V: rows behind the sequence become zeros, elements of drafted tokens that are not finite too.  A tile that both streams read
-          // is shared out, and neither stream's P V starts before it is done.
+          // is shared out, and neither stream's P V starts before it is done; half tiles are each stream's own.
           const uint32_t r = 2 * (gt + i) + 1;
           uint8_t* v = ring + (r % kSlots) * kSlotBytes;
-          ok = __all_sync(0xffffffffu, tile_there(r));
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[r % kSlots], (r / kSlots) & 1, deadline));
           if (!ok) break;
           const int who = MT == 2 ? tid : row;
-          for (int tok = max(committed - tok0, 0) + (who >> 4); tok < kTile; tok += 8 * MT) {
+          for (int tok = max(committed - tok0, first) + (who >> 4); tok < first + kHere; tok += 8 * MT) {
             uint4* at = reinterpret_cast<uint4*>(v + ((row >> 3) & 1) * kHalf + swz128(tok, row & 7));
             uint4 x = make_uint4(0, 0, 0, 0);
             if (tok0 + tok < seg.len) {
@@ -381,9 +370,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
           if (special) {
             // masked scores become -inf where they lie; what is rare is kept in short loops, for the sake of the instruction cache
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t seen = mask_bits(words, p.words, tok0 + 32 * c - committed);
-              const int left = seg.len - tok0 - 32 * c;
+            for (int c = 0; c < kChunks; ++c) {
+              uint32_t seen = mask_bits(words, p.words, tok0 + first + 32 * c - committed);
+              const int left = seg.len - tok0 - first - 32 * c;
               if (left < 32) seen &= left <= 0 ? 0u : (1u << left) - 1u;
               uint32_t x[32];
               tmem_ld_x32(tq + col_s + 32 * c, x);
@@ -395,9 +384,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             }
             tmem_st_wait();
           }
-          uint32_t v[4][32];
+          uint32_t v[kChunks][32];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
+          for (int c = 0; c < kChunks; ++c) tmem_ld_x32(tq + col_s + 32 * c, v[c]);
           tmem_ld_wait();
           // The exponentials are what a step is made of (16 a cycle and SM: 1024 cycles a tile).  Two streams that start on the same KV tile
           // would stay in step, both at their exponentials and then both waiting for the tensor cores, so they take turns.
@@ -428,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             if (huge && f2.x != 1.f) {
               f2 = make_float2(1.f, 1.f);
 #pragma unroll
-              for (int c = 0; c < 4; ++c)
+              for (int c = 0; c < kChunks; ++c)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[c][j] = __float_as_uint(__uint_as_float(v[c][j]) * sl2);
             }
@@ -437,11 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             if (again) break;
             float mx[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = max_nan(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
+            for (int c = 0; c < 4; ++c) mx[c] = max_nan(__uint_as_float(v[c % kChunks][c]), __uint_as_float(v[c % kChunks][c + 4]));
 #pragma unroll
-            for (int j = 2; j < 32; j += 2)
+            for (int j = 0; j < 32; j += 2)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) mx[c] = max_nan(mx[c], __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
+              for (int c = 0; c < kChunks; ++c) mx[(c + j) & 3] = max_nan(mx[(c + j) & 3], __uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1]));
             // a NaN or +inf among the scores makes the row's maximum NaN, and so all that is computed with it
             float top = max_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]) * f2.x - kBias;
             if (top == INFINITY) top = __int_as_float(0x7fffffff);
@@ -453,8 +442,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             l *= alpha;
             m = m_new;
             tmem_st_wait();                        // the half that will be done again
-            if (k > 0) {
-              // the scores' commit covers the P V before them: O is complete
+            if (i > 0) {
+              if (MT == 1) {
+                // scores come a tile early here; O is complete when V of the tile before has been read (its place in the ring was given out
+                // before that of the K whose scores are here, so the parity is the right one)
+                const uint32_t r = 2 * (gt + i) - 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(&kv_free[r % kSlots], (r / kSlots) & 1, deadline));
+                if (!ok) break;
+                tc_fence_after_sync();
+              }
+              // two row tiles: the scores' commit covers the P V before them, O is complete
 #pragma unroll 1
               for (int c0 = 0; c0 < kD; c0 += 16) {
                 uint32_t x[16];
@@ -470,41 +467,42 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
             // Beyond, the products are rounded too, or the factor could overflow.
             huge |= __any_sync(0xffffffffu, fabsf(mn) > 16777216.f) != 0;
           }
+          if (!ok) break;
           tmem_st_wait();
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[st][0]);
+          // (one row tile: by turns, because a warp may be a tile ahead of its neighbours)
+          if (lane == 0) mbar_arrive(&p_full[st][MT == 1 ? buf : 0]);
           if (MT == 2 && lane == 0) mbar_arrive(&turn[st ^ 1]);
-          half_chunk(2, make_float2(mn, mn));
-          half_chunk(3, make_float2(mn, mn));
-          tmem_st_wait();
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[st][1]);
+          if constexpr (MT == 2) {
+            half_chunk(2, make_float2(mn, mn));
+            half_chunk(3, make_float2(mn, mn));
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[st][1]);
+          }
           l += sum.x + sum.y;
         } else {
           if (MT == 2) ok = __all_sync(0xffffffffu, mbar_wait(&turn[st], (steps & 1) ^ (st == 0 ? 1 : 0), deadline));
           if (!ok) break;
           if (lane == 0) {
-            mbar_arrive(&p_full[st][0]);
-            mbar_arrive(&p_full[st][1]);
-            if (MT == 2) mbar_arrive(&turn[st ^ 1]);
+            mbar_arrive(&p_full[st][MT == 1 ? buf : 0]);
+            if (MT == 2) {
+              mbar_arrive(&p_full[st][1]);
+              mbar_arrive(&turn[st ^ 1]);
+            }
           }
         }
       }
 
       // ---- the next segment's Q, while this one's last products run: its place is not read any more ------------
-      // (a stream without steps has not heard of its MMA warp: neither may be a phase of q_full ahead of the other)
-      if (n_steps == 0) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&idle, n_idle & 1, deadline));
-        ++n_idle;
-      }
       Segment nx;
       more = ok && walk.next(p, nx);
       if (more) load_q(nx, n_seg + 1);
 
       // ---- join the streams -------------------------------------------------------------------------------------
-      const bool both = MT == 1 && seg.count > 1;
+      constexpr bool both = MT == 1;
       float f0, f1 = 0.f, M = m, L = l;
       if (MT == 1) {
         if (st == 1) {
@@ -513,11 +511,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
         }
         bar_sync_named(1, 32 * kSmWarps);
         if (st == 0) {
-          const float m1 = both ? s_x[0][row] : -INFINITY;
+          const float m1 = s_x[0][row];
           M = max_nan(m, m1);
           f0 = m == -INFINITY ? 0.f : fast_exp2(m - M);
           f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - M);
-          L = l * f0 + (both ? s_x[1][row] * f1 : 0.f);
+          L = l * f0 + s_x[1][row] * f1;
           const float inv = L == 0.f ? 0.f : 1.f / L;                // a NaN stays one
           f0 *= inv;
           f1 *= inv;
@@ -533,8 +531,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
         f0 = L == 0.f ? 0.f : 1.f / L;
       }
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[MT == 2 ? st : 0], n_seg & 1, deadline));
-      if (ok && both) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[1], n_joined & 1, deadline));
-      n_joined += both;
       tc_fence_after_sync();
 
       // ---- write the result or a piece ----------------------------------------------------------------------------
@@ -636,7 +632,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
           if (r >= (uint32_t)kSlots) ok = __all_sync(0xffffffffu, mbar_wait(&kv_free[slot], (r / kSlots - 1) & 1, deadline));
           if (!ok) break;
           if (lane == 0) {
-            if (lw == 0) *reinterpret_cast<volatile uint32_t*>(&s_issued) = r + 1;
             mbar_expect_tx(&kv_full[slot], (uint32_t)mine * p.box_tok * kD);
           }
           __syncwarp();
@@ -663,7 +658,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     }
   } else if (warp >= kMmaWarp) {
     // =========================== MMA issue ===========================
-    // A warp per stream: one warp for both, in a fixed order, held a stream up behind the other (128k tokens, 64 drafted 315 us).
     // rows that no unit covers: those of sequences without a token here, and those behind the last sequence
     if (warp == kMmaWarp) {
       auto clear = [&](int r0, int r1) {
@@ -682,86 +676,104 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     const uint64_t d_q = umma_desc_k_sw128(smem_u32(smem)), d_k = umma_desc_k_sw128(smem_u32(ring)),
                    d_v = umma_desc_mn_sw128(smem_u32(ring), kHalf);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0; };
-    // (the stream is a constant of the code, so that the columns are: an operand that is not known to be the same in all lanes costs
-    // an MMA some 100 cycles)
-    auto role = [&](auto stream) {
-    constexpr int st = decltype(stream)::value;
-    constexpr uint32_t col_s = kColS + 128 * st, col_o = kColO + 128 * st;
-    uint32_t steps = 0, n_seg = 0, q_at = 0;
-    auto k_there = [&](int i_lane) {
-      const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0);
-      return __all_sync(0xffffffffu, tile_there(r)) != 0;
-    };
-    auto scores = [&](int i_lane) {                // S of tile i, which is there
-      const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0), slot = r % kSlots;
+    auto tile_there = [&](uint32_t r) { return wait(&kv_full[r % kSlots], (r / kSlots) & 1); };
+    // scores of a tile that is there: S, 128 columns, and its commits
+    auto scores = [&](uint32_t col, uint32_t qb, uint32_t r, uint64_t* done) {
       tc_fence_after_sync();
-      const uint32_t kb = slot * kSlotBytes, qb = q_at;
+      const uint32_t kb = r % kSlots * kSlotBytes;
       if (elect_one()) {
 #pragma unroll
         for (int ks = 0; ks < kD / 16; ++ks) {
           const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
-          umma_bf16(col_s, d_q + ((qb + off) >> 4), d_k + ((kb + off) >> 4), id_s, ks > 0);
+          umma_bf16(col, d_q + ((qb + off) >> 4), d_k + ((kb + off) >> 4), id_s, ks > 0);
         }
-        umma_commit(&s_full[st]);
-        umma_commit(&kv_free[slot]);
+        umma_commit(done);
+        umma_commit(&kv_free[r % kSlots]);
       }
       __syncwarp();
-      return true;
     };
-    auto values = [&](int i_lane, int k_lane, int next) {  // O += P V of tile i
-      const uint32_t r = 2 * __shfl_sync(0xffffffffu, gt + i_lane, 0) + 1, later = __shfl_sync(0xffffffffu, k_lane, 0), slot = r % kSlots;
-      // V first: what is there already still takes a wait's time, which is better spent before P is there
-      if (__all_sync(0xffffffffu, tile_there(r)) == 0 || !wait(&p_full[st][0], steps & 1)) return false;
+    // O += P V for 64 tokens of a tile
+    auto values = [&](uint32_t col_o, uint32_t col_p, uint32_t r, int tok, uint32_t later) {
       tc_fence_after_sync();
-      const uint32_t v_lo = (uint32_t)d_v + (slot * kSlotBytes >> 4), v_hi = (uint32_t)(d_v >> 32);
+      const uint32_t v_lo = (uint32_t)d_v + ((r % kSlots * kSlotBytes + tok * 128) >> 4), v_hi = (uint32_t)(d_v >> 32);
       if (elect_one()) {
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          if (ks == 0) umma_bf16_ts_first(col_o, col_s, v_lo, v_hi, id_o, later);
-          else umma_bf16_ts(col_o, col_s + 8 * ks, v_lo + ks * 128, v_hi, id_o);
+          if (ks == 0) umma_bf16_ts_first(col_o, col_p, v_lo, v_hi, id_o, later);
+          else umma_bf16_ts(col_o, col_p + 8 * ks, v_lo + ks * 128, v_hi, id_o);
         }
       }
       __syncwarp();
-      // two row tiles: the next K is there by now, and is looked for while P is not.  One: the cache may be what everything waits for,
-      // and this V's place is needed
-      if ((MT == 2 && next >= 0 && !k_there(next)) || !wait(&p_full[st][1], steps & 1)) return false;
-      ++steps;
-      tc_fence_after_sync();
-      if (elect_one()) {
-#pragma unroll
-        for (int ks = 4; ks < 8; ++ks) umma_bf16_ts(col_o, col_s + 8 * ks, v_lo + ks * 128, v_hi, id_o);
-        umma_commit(&kv_free[slot]);
-      }
-      __syncwarp();
-      return true;
     };
-    while (ok && walk.next(p, seg)) {
-      q_at = (__shfl_sync(0xffffffffu, MT == 2 ? (uint32_t)st : n_seg, 0) & 1) * kSlotBytes;
-      const int n = MT == 2 ? seg.count : (seg.count - st + 1) / 2;
-      ok = wait(&q_full, n_seg & 1);
-      ++n_seg;
-      if (!ok) break;
-      tc_fence_after_sync();
-      auto tile = [&](int k) { return MT == 2 ? k : 2 * k + st; };
-      if (n > 0) ok = k_there(tile(0)) && scores(tile(0));
-      for (int k = 0; k < n && ok; ++k) {
-        ok = values(tile(k), k, k + 1 < n ? tile(k + 1) : -1);
-        if (ok && k + 1 < n) ok = (MT == 2 || k_there(tile(k + 1))) && scores(tile(k + 1));
+    uint32_t n_seg = 0, steps = 0;
+    if constexpr (MT == 1) {
+      // One warp: scores of the next but one tile follow the P V that frees their place.
+      if (warp == kMmaWarp) {
+        while (ok && walk.next(p, seg)) {
+          const uint32_t qb = (__shfl_sync(0xffffffffu, n_seg, 0) & 1) * kSlotBytes;
+          ok = wait(&q_full, n_seg & 1);
+          ++n_seg;
+          for (int i_lane = -2; i_lane < seg.count && ok; ++i_lane) {
+            // through a shuffle: what is computed from it is then known to be the same in all lanes and stays in uniform registers,
+            // where the MMA reads its operands (moving them there costs some 100 cycles each)
+            const int i = __shfl_sync(0xffffffffu, i_lane, 0);
+            const uint32_t tile = __shfl_sync(0xffffffffu, gt, 0) + i, r = 2 * tile + 1;
+            if (i >= 0) {
+              ok = tile_there(r);
+              for (int st = 0; st < 2 && ok; ++st) {
+                ok = wait(&p_full[st][tile & 1], (tile >> 1) & 1);
+                if (!ok) break;
+                values(kColO + 128 * st, kColS + 128 * (tile & 1) + 64 * st, r, 64 * st, i);
+              }
+              if (ok && elect_one()) umma_commit(&kv_free[r % kSlots]);
+              __syncwarp();
+            }
+            if (ok && i + 2 < seg.count) {
+              ok = tile_there(r + 3);
+              if (ok) scores(kColS + 128 * (tile & 1), qb, r + 3, &s_full[tile & 1]);
+            }
+          }
+          if (ok && elect_one()) umma_commit(&o_full[0]);
+          __syncwarp();
+          gt += seg.count;
+        }
       }
-      if (ok && elect_one()) {
-        if (n > 0) umma_commit(&o_full[st]);
-        else mbar_arrive(&idle);
-      }
-      __syncwarp();
-      gt += seg.count;
+    } else {
+      // A warp per stream: one warp for both, in a fixed order, held a stream up behind the other (128k tokens, 64 drafted 315 us).  (The
+      // stream is a constant of the code, so that the columns are.)
+      auto role = [&](auto stream) {
+        constexpr int st = decltype(stream)::value;
+        while (ok && walk.next(p, seg)) {
+          ok = wait(&q_full, n_seg & 1);
+          ++n_seg;
+          if (ok && (ok = tile_there(2 * __shfl_sync(0xffffffffu, gt, 0)))) scores(kColS + 128 * st, st * kSlotBytes, 2 * __shfl_sync(0xffffffffu, gt, 0), &s_full[st]);
+          for (int i_lane = 0; i_lane < seg.count && ok; ++i_lane, ++steps) {
+            const int i = __shfl_sync(0xffffffffu, i_lane, 0);
+            const uint32_t r = 2 * (__shfl_sync(0xffffffffu, gt, 0) + i) + 1;
+            // V first, and the next K before the second half: what is there already still takes a wait's time
+            ok = tile_there(r) && wait(&p_full[st][0], steps & 1);
+            if (!ok) break;
+            values(kColO + 128 * st, kColS + 128 * st, r, 0, i);
+            if (i + 1 < seg.count) ok = tile_there(r + 1);
+            if (!ok || !(ok = wait(&p_full[st][1], steps & 1))) break;
+            values(kColO + 128 * st, kColS + 128 * st + 32, r, 64, 1);
+            if (elect_one()) umma_commit(&kv_free[r % kSlots]);
+            __syncwarp();
+            if (i + 1 < seg.count) scores(kColS + 128 * st, st * kSlotBytes, r + 1, &s_full[st]);
+          }
+          if (ok && elect_one()) umma_commit(&o_full[st]);
+          __syncwarp();
+          gt += seg.count;
+        }
+      };
+      if (warp == kMmaWarp) role(std::integral_constant<int, 0>{});
+      else role(std::integral_constant<int, 1>{});
     }
     if (!ok) {
-      if (elect_one()) umma_commit(&drain[st]);    // nothing of this CTA's may be in flight when it leaves
-      mbar_wait(&drain[st], 0, now_ns() + 10000000ull);
+      uint64_t* const mine = &drain[warp - kMmaWarp];
+      if (elect_one()) umma_commit(mine);          // nothing of this CTA's may be in flight when it leaves
+      mbar_wait(mine, 0, now_ns() + 10000000ull);
     }
-    };
-    if (warp == kMmaWarp) role(std::integral_constant<int, 0>{});
-    else role(std::integral_constant<int, 1>{});
   }
   if (!ok && lane == 0) atomicCAS(p.error_flag, 0, (int)kTimeoutMbarrier);
 
