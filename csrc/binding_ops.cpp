@@ -282,17 +282,20 @@ std::tuple<torch::Tensor, torch::Tensor> tree_decode(torch::Tensor q, torch::Ten
   }
   helix::TreeDecodeParams p{};
   p.box_tok = page % 128 == 0 ? 128 : page % 64 == 0 ? 64 : page % 32 == 0 ? 32 : 16;
-  auto map = [&](const torch::Tensor& c, CUtensorMap* m) {
-    const uint64_t dims[4] = {128, (uint64_t)page, (uint64_t)Hkv, (uint64_t)pages};
-    const uint64_t strides[3] = {(uint64_t)c.stride(td) * 2, (uint64_t)c.stride(hd) * 2, (uint64_t)c.stride(0) * 2};
-    const uint32_t box[4] = {64, (uint32_t)p.box_tok, 1, 1};
+  // K as 4-D, V with the halves of head_dim as a dimension of their own
+  auto map = [&](const torch::Tensor& c, CUtensorMap* m, bool halves) {
+    const uint64_t tok = (uint64_t)c.stride(td) * 2, head = (uint64_t)c.stride(hd) * 2, pg = (uint64_t)c.stride(0) * 2;
+    const uint64_t dims4[4] = {128, (uint64_t)page, (uint64_t)Hkv, (uint64_t)pages}, strides4[3] = {tok, head, pg};
+    const uint64_t dims5[5] = {64, (uint64_t)page, 2, (uint64_t)Hkv, (uint64_t)pages}, strides5[4] = {tok, 128, head, pg};
+    const uint32_t box4[4] = {64, (uint32_t)p.box_tok, 1, 1}, box5[5] = {64, (uint32_t)p.box_tok, 2, 1, 1};
     const char* err = nullptr;
-    TORCH_CHECK(helix::encode_tensor_map(m, type == at::ScalarType::Half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                                         c.data_ptr(), dims, strides, box, helix::TmaSwizzle::k128B, &err),
+    TORCH_CHECK(helix::encode_tensor_map(m, type == at::ScalarType::Half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                         halves ? 5 : 4, c.data_ptr(), halves ? dims5 : dims4, halves ? strides5 : strides4, halves ? box5 : box4,
+                                         helix::TmaSwizzle::k128B, &err),
                 "helix: KV cache tensor map: ", err ? err : "?");
   };
-  map(k_cache, &p.k_map);
-  map(v_cache, &p.v_map);
+  map(k_cache, &p.k_map, false);
+  map(v_cache, &p.v_map, true);
   const int group = (int)(Hq / Hkv), sms = helix::device_sm_count();
   const int max_q = (int)(max_q_len > 0 ? std::min(max_q_len, rows) : rows), longest = (int)std::min<int64_t>(std::max<int64_t>(max_seq_len, 1), 0x7fffff00);
   const helix::TreePlan plan = helix::tree_plan((int)B, (int)Hkv, group, max_q, longest, sms);

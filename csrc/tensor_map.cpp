@@ -29,9 +29,9 @@ bool encode_tensor_map(CUtensorMap* out, CUtensorMapDataType dtype, int rank, co
     if (err) *err = "TMA base address must be 16-byte aligned";
     return false;
   }
-  cuuint64_t gdims[4];
-  cuuint64_t gstrides[3];
-  cuuint32_t gbox[4], estr[4];
+  cuuint64_t gdims[5];
+  cuuint64_t gstrides[4];
+  cuuint32_t gbox[5], estr[5];
   for (int i = 0; i < rank; ++i) {
     gdims[i] = dims[i];
     gbox[i] = box[i];

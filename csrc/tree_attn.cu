@@ -37,7 +37,7 @@ namespace {
 using namespace sm100;
 
 constexpr int kD = 128, kTile = 128, kRows = 128;
-constexpr int kSlotBytes = kTile * kD * 2;             // 32768: one K or V tile, two halves of [128 tokens x 64 dims]
+constexpr int kSlotBytes = kTile * kD * 2;             // 32768: one K tile, two halves of [128 tokens x 64 dims], or V tile (v_at)
 constexpr int kHalf = kTile * 128;                     // 16384
 constexpr int kSmWarps = 8, kMmaWarp = 8, kFirstLoad = 10, kLoadWarps = 2, kThreads = 384;      // an MMA warp per stream
 constexpr int kSlots = 5;                              // beside two tiles of Q
@@ -164,6 +164,9 @@ struct Walk {
   }
 };
 
+// Where token `tok` of a V tile begins, dims 0 ... 63 (before the swizzle): boxes of 2^shift tokens, both halves of the dims in each
+__device__ __forceinline__ uint32_t v_at(int tok, int shift) { return ((tok >> shift) << (shift + 8)) + (tok & ((1 << shift) - 1)) * 128; }
+
 // 32 visibility bits from drafted token `off` on (negative: committed ones before the first) of a row's mask words
 __device__ __forceinline__ uint32_t mask_bits(const uint64_t* words, int n_words, int off) {
   if (off <= -32) return 0xffffffffu;
@@ -186,6 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
   int* s_base = reinterpret_cast<int*>(smem);      // [kSeqTable] first place of each sequence on the line, until Q comes
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.Hq / p.Hkv;
+  const int box_shift = 31 - __clz(p.box_tok);
 
   if (tid == 0) {
     for (int i = 0; i < kSlots; ++i) {
@@ -339,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
           if (!ok) break;
           const int who = MT == 2 ? tid : row;
           for (int tok = max(committed - tok0, first) + (who >> 4); tok < first + kHere; tok += 8 * MT) {
-            uint4* at = reinterpret_cast<uint4*>(v + ((row >> 3) & 1) * kHalf + swz128(tok, row & 7));
+            // (rows of 128 bytes, boxes of whole groups of eight: the swizzle goes by the token)
+            uint4* at = reinterpret_cast<uint4*>(v + v_at(tok, box_shift) + ((row >> 3) & 1) * (p.box_tok * 128) + (((row & 7) ^ (tok & 7)) << 4));
             uint4 x = make_uint4(0, 0, 0, 0);
             if (tok0 + tok < seg.len) {
               x = *at;
@@ -610,9 +615,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
   }
   if (warp >= kFirstLoad) {
     // =========================== loads ===========================
-    // Boxes of 16 tokens x 64 dims (a page of 16 tokens allows no larger ones): 32 per tile, shared by two warps, each issued by
-    // one elected lane of a warp that has stayed together.  One warp whose lanes issued a box each took ~136 cycles per box,
-    // 4400 per tile, which bounded everything (64 x 8192 tokens 528 us).
+    // With pages of 16 tokens a tile is many small boxes, and a box costs the copy engine ~100 cycles whatever its size: 32 boxes of
+    // 2 KB per tile, as K still has them, bounded everything (1 x 128k tokens, 16 drafted 141 us).  V, whose layout the MMA takes 16 tokens
+    // at a time, comes with both halves of the dims in one box.
     const int per_tile = kTile / p.box_tok, lw = warp - kFirstLoad;
     uint32_t issued = 0;
     while (ok && walk.next(p, seg)) {
@@ -624,22 +629,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       int page = page_at(0);
       for (int i = 0; i < seg.count && ok; ++i) {
         const int tok0 = (seg.t_begin + i) * kTile, in_page = (tok0 + lane * p.box_tok) % p.page_size;
-        const int boxes = 2 * ((min(seg.len - tok0, kTile) + p.box_tok - 1) / p.box_tok);
-        const int mine = (boxes - lw + kLoadWarps - 1) / kLoadWarps;
+        const int blocks = (min(seg.len - tok0, kTile) + p.box_tok - 1) / p.box_tok;
         const int next = page_at(i + 1);
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t r = 2 * (gt + i) + kv, slot = r % kSlots;
           if (r >= (uint32_t)kSlots) ok = __all_sync(0xffffffffu, mbar_wait(&kv_free[slot], (r / kSlots - 1) & 1, deadline));
           if (!ok) break;
-          if (lane == 0) {
-            mbar_expect_tx(&kv_full[slot], (uint32_t)mine * p.box_tok * kD);
-          }
+          // K: a box per half of the dims, the halves shared by the two warps.  V: boxes of both halves, every other block.
+          const int mine = kv == 0 ? blocks : (blocks - lw + kLoadWarps - 1) / kLoadWarps;
+          if (lane == 0) mbar_expect_tx(&kv_full[slot], (uint32_t)mine * p.box_tok * (kv == 0 ? kD : 2 * kD));
           __syncwarp();
-          for (int j = lw; j < boxes; j += kLoadWarps) {
-            const int pg = __shfl_sync(0xffffffffu, page, j >> 1), at = __shfl_sync(0xffffffffu, in_page, j >> 1), half = j & 1;
-            if (elect_one())
-              tma_load_4d(ring + slot * kSlotBytes + half * kHalf + (j >> 1) * p.box_tok * 128, kv == 0 ? &p.k_map : &p.v_map,
-                          &kv_full[slot], 64 * half, at, seg.kvh, pg);
+          for (int j = kv == 0 ? 0 : lw; j < blocks; j += kv == 0 ? 1 : kLoadWarps) {
+            const int pg = __shfl_sync(0xffffffffu, page, j), at = __shfl_sync(0xffffffffu, in_page, j);
+            if (elect_one()) {
+              uint8_t* dst = ring + slot * kSlotBytes;
+              if (kv == 0) tma_load_4d(dst + lw * kHalf + j * p.box_tok * 128, &p.k_map, &kv_full[slot], 64 * lw, at, seg.kvh, pg);
+              else tma_load_5d(dst + j * p.box_tok * 256, &p.v_map, &kv_full[slot], 0, at, 0, seg.kvh, pg);
+            }
             __syncwarp();
           }
           issued = r + 1;
@@ -674,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     constexpr uint32_t id_s = fmt, id_o = fmt | (1u << 16);          // V is MN-major
     // all 512 columns are this CTA's: tensor memory starts at column 0, and no register holds the base
     const uint64_t d_q = umma_desc_k_sw128(smem_u32(smem)), d_k = umma_desc_k_sw128(smem_u32(ring)),
-                   d_v = umma_desc_mn_sw128(smem_u32(ring), kHalf);
+                   d_v = umma_desc_mn_sw128(smem_u32(ring), p.box_tok * 128);
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0; };
     auto tile_there = [&](uint32_t r) { return wait(&kv_full[r % kSlots], (r / kSlots) & 1); };
     // scores of a tile that is there: S, 128 columns, and its commits
@@ -695,12 +701,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     // O += P V for 64 tokens of a tile
     auto values = [&](uint32_t col_o, uint32_t col_p, uint32_t r, int tok, uint32_t later) {
       tc_fence_after_sync();
-      const uint32_t v_lo = (uint32_t)d_v + ((r % kSlots * kSlotBytes + tok * 128) >> 4), v_hi = (uint32_t)(d_v >> 32);
+      const uint32_t v_lo = (uint32_t)d_v + (r % kSlots * kSlotBytes >> 4), v_hi = (uint32_t)(d_v >> 32);
       if (elect_one()) {
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          if (ks == 0) umma_bf16_ts_first(col_o, col_p, v_lo, v_hi, id_o, later);
-          else umma_bf16_ts(col_o, col_p + 8 * ks, v_lo + ks * 128, v_hi, id_o);
+          const uint32_t lo = v_lo + (v_at(tok + 16 * ks, box_shift) >> 4);
+          if (ks == 0) umma_bf16_ts_first(col_o, col_p, lo, v_hi, id_o, later);
+          else umma_bf16_ts(col_o, col_p + 8 * ks, lo, v_hi, id_o);
         }
       }
       __syncwarp();

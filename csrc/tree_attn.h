@@ -8,7 +8,8 @@
 namespace helix {
 
 struct TreeDecodeParams {
-  CUtensorMap k_map, v_map;        // 4-D (d, token in page, kv head, page), box (64, box_tok, 1, 1), SWIZZLE_128B
+  CUtensorMap k_map;               // 4-D (d, token in page, kv head, page), box (64, box_tok, 1, 1), SWIZZLE_128B
+  CUtensorMap v_map;               // 5-D (d % 64, token in page, d / 64, kv head, page), box (64, box_tok, 2, 1, 1), SWIZZLE_128B
   const uint16_t* q;               // [rows, Hq, 128] bf16 or fp16
   int64_t q_sr, q_sh;              // elements
   const uint16_t* v;               // the V cache itself, for values that are not finite
