@@ -9,6 +9,10 @@ One decode step of the attention block of every layer on one CP rank::
 The KV cache of every sequence is split evenly over the ``cp_size`` ranks; each rank holds all KV
 heads of its shard.  Weights are random-init (N(0, 0.02)), KV ~ N(0, 1): there is no checkpoint
 loading here, the stack exists to drive and measure the kernels on the shapes of a real model.
+
+With ``draft_tokens`` the stack also verifies drafted tokens (:meth:`HelixDecodeStack.verify_step`): the step's new tokens of all sequences
+get their pages and slots on the device, their K and V go into this rank's part of the cache, every token attends to the cache and
+to its ancestors in the tree, and :meth:`HelixDecodeStack.commit` keeps those that were accepted.
 The reference leaves all of this to vLLM (``benchmark/sbatch/run_gb200_aiperf_v3.sbatch:284-305``).
 """
 from __future__ import annotations
@@ -21,7 +25,7 @@ import torch
 import torch.distributed as dist
 
 from .. import api
-from ..ops import attention, oproj as oproj_mod
+from ..ops import attention, oproj as oproj_mod, paged
 from ..ops._ext import ext
 from ..utils import env
 from ..utils.tracing import nvtx_range
@@ -54,7 +58,9 @@ class HelixDecodeStack:
     def __init__(self, cfg: LlamaDecodeConfig, *, batch: int, local_ctx: int, cp_size: int = 1, cp_rank: int = 0,
                  group: Optional[dist.ProcessGroup] = None, device="cuda", seed: int = 0,
                  workspace: Optional[torch.Tensor] = None, kv_std: float = 1.0,
-                 fuse_oproj: Optional[bool] = False):
+                 fuse_oproj: Optional[bool] = False, draft_tokens: int = 0, w_bits: int = 16):
+        """``draft_tokens``: most tokens of one sequence that :meth:`verify_step` and :meth:`commit` will ever add (pages are set aside
+        for them); ``w_bits=4`` keeps the o_proj weights in 4 bits with a scale per 128 columns."""
         assert cfg.n_q_heads % cp_size == 0, "query heads must divide evenly over the CP ranks"
         self.cfg, self.batch, self.local_ctx = cfg, batch, local_ctx
         self.cp_size, self.cp_rank, self.group = cp_size, cp_rank, group
@@ -64,17 +70,29 @@ class HelixDecodeStack:
         # (a request that does not fit runs the two-kernel chain, and is counted as such)
         fits = cp_size > 1 and self.device.type == "cuda" and api.alltoall_combine_oproj_fits(
             batch, self.heads_local, cfg.head_dim, cfg.hidden, cp_size)
-        self.fuse_oproj = bool(fits) if fuse_oproj is None else bool(fuse_oproj and fits)
+        self.fuse_oproj = (bool(fits) if fuse_oproj is None else bool(fuse_oproj and fits)) and w_bits == 16
         self.k_local = self.heads_local * cfg.head_dim
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
         gen = torch.Generator(device=self.device)
         gen.manual_seed(seed * 1000 + cp_rank)
         pages_per_seq = (local_ctx + cfg.page_size - 1) // cfg.page_size
-        self.n_pages = batch * pages_per_seq
+        if w_bits not in (4, 16):
+            raise ValueError("w_bits must be 4 or 16")
+        self.w_bits = w_bits
+        self.draft_tokens = draft_tokens
+        spare = batch * ((draft_tokens + cfg.page_size - 1) // cfg.page_size + 1) if draft_tokens else 0
+        self.n_pages = batch * pages_per_seq + spare
         # pages of a sequence are scattered over the pool, as a paged allocator would leave them
         perm = torch.randperm(self.n_pages, generator=torch.Generator().manual_seed(seed)).int()
-        self.block_table = perm.view(batch, pages_per_seq).to(self.device)
+        owned = perm[:batch * pages_per_seq].view(batch, pages_per_seq)
+        self.block_table = torch.nn.functional.pad(owned, (0, spare // batch if spare else 0)).to(self.device)
         self.seq_lens = torch.full((batch,), local_ctx, dtype=torch.int32, device=self.device)
+        self.max_local = self.block_table.shape[1] * cfg.page_size if draft_tokens else local_ctx
+        # state of ops.paged.extend_tables: the pages each sequence holds, the free ones, committed tokens over all ranks
+        self.held = torch.full((batch,), pages_per_seq, dtype=torch.int32, device=self.device)
+        self.free_pages = perm[batch * pages_per_seq:].to(self.device)
+        self.free_used = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.ctx_lens = torch.full((batch,), local_ctx * cp_size, dtype=torch.int32, device=self.device)
         shape = (self.n_pages, cfg.n_kv_heads, cfg.page_size, cfg.head_dim)
         self.k_cache: List[torch.Tensor] = []
         self.v_cache: List[torch.Tensor] = []
@@ -105,7 +123,7 @@ class HelixDecodeStack:
     def layer(self, l: int, q: torch.Tensor) -> torch.Tensor:
         with nvtx_range(f"layer{l}.attention"):
             o, lse = attention.gqa_decode(q, self.k_cache[l], self.v_cache[l], self.block_table, self.seq_lens,
-                                          scale=self.scale, max_seq_len=self.local_ctx, kv_stable=True)
+                                          scale=self.scale, max_seq_len=self.max_local, kv_stable=True)
         if self.cp_size > 1 and self.fuse_oproj:
             # exchange + combine + o_proj in one launch: W_o streams while the exchange is in flight
             return api.alltoall_combine_oproj(o, lse, self._oproj_weight(l), self.workspace, self.cp_rank, self.cp_size)
@@ -119,6 +137,10 @@ class HelixDecodeStack:
         """The layer's o_proj weight in the layout the GEMM streams fastest: packed once, on first use
         (one contiguous bulk copy per pipeline stage instead of strided tensor copies); the plain matrix
         stays in ``w_o`` for the one-kernel path and for oracles.  ``prepack_oproj=False`` keeps the plain one."""
+        if self.w_bits == 4:
+            if self._w_o_packed[l] is None:
+                self._w_o_packed[l] = oproj_mod.quantize_weight_int4(self.w_o[l], 128)
+            return self._w_o_packed[l]
         if not self.prepack_oproj or not self.w_o[l].is_cuda or self.w_o[l].shape[0] % 128 or self.w_o[l].shape[1] % 64:
             return self.w_o[l]
         if self._w_o_packed[l] is None:
@@ -138,6 +160,44 @@ class HelixDecodeStack:
 
     def _step_last(self, q_all: torch.Tensor) -> torch.Tensor:
         return self._run_layers(q_all, 0, self.cfg.n_layers)
+
+    # ---- drafted tokens ---------------------------------------------------------------------------
+    def _extend(self, q_start: torch.Tensor, rows: int, parents, mask_words: int) -> paged.TablePlan:
+        return paged.extend_tables(self.block_table, self.held, self.free_pages, self.free_used, self.ctx_lens, q_start, rows=rows,
+                                   page_size=self.cfg.page_size, parents=parents, mask_words=mask_words, cp_size=self.cp_size,
+                                   cp_rank=self.cp_rank)
+
+    def verify_step(self, q_all: torch.Tensor, k_all: torch.Tensor, v_all: torch.Tensor, q_start: torch.Tensor,
+                    parents: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One pass over drafted tokens: ``q_all [L, rows, Hq, D]``, ``k_all`` / ``v_all [L, rows, Hkv, D]``, rows ``q_start[b]`` to
+        ``q_start[b + 1]`` are sequence ``b``'s, ``parents [rows]`` their tree (``None``: chains); see :func:`ops.paged.extend_tables`.
+        Returns ``y [L, rows, hidden]`` (this rank's partial sums).  Committed lengths stay as they are: the next call overwrites
+        the drafted tokens, unless :meth:`commit` keeps some.  No host synchronisation, so the step can be captured."""
+        if not self.draft_tokens:
+            raise RuntimeError("this stack was made without draft_tokens")
+        rows = q_all.shape[1]
+        words = min((self.draft_tokens + 63) // 64, 4)
+        plan = self._extend(q_start, rows, parents, words)
+        ys = []
+        for l in range(self.cfg.n_layers):
+            paged.append_kv(k_all[l], v_all[l], self.k_cache[l], self.v_cache[l], plan.slots)
+            with nvtx_range(f"layer{l}.tree_attention"):
+                o, lse = attention.tree_decode(q_all[l], self.k_cache[l], self.v_cache[l], self.block_table, plan.seq_lens, q_start,
+                                               plan.draft_lens, plan.mask, scale=self.scale, max_seq_len=self.max_local, max_q_len=self.draft_tokens)
+            x = api.alltoall_combine(o, lse, self.workspace, self.cp_rank, self.cp_size) if self.cp_size > 1 else o
+            ys.append(oproj_mod.oproj(x.reshape(rows, self.k_local), self._oproj_weight(l)))
+        return torch.stack(ys)
+
+    def commit(self, k_all: torch.Tensor, v_all: torch.Tensor, accepted: torch.Tensor, q_start: torch.Tensor) -> None:
+        """Keep drafted tokens: ``accepted`` are their rows in ``k_all`` / ``v_all``, in the order of their positions, and ``q_start [B + 1]``
+        says which of them belong to which sequence.  A path through a tree becomes a run of tokens behind the committed ones."""
+        if not self.draft_tokens:
+            raise RuntimeError("this stack was made without draft_tokens")
+        plan = self._extend(q_start, accepted.numel(), None, 0)
+        for l in range(self.cfg.n_layers):
+            paged.append_kv(k_all[l][accepted], v_all[l][accepted], self.k_cache[l], self.v_cache[l], plan.slots)
+        self.ctx_lens += q_start.diff()
+        self.seq_lens.copy_(plan.seq_lens)
 
     # ---- end-to-end call: pinned host input -> host output ---------------------------------------
     def capture(self, q_example: torch.Tensor, head_layers: Optional[int] = None) -> None:
@@ -219,6 +279,8 @@ class HelixDecodeStack:
         attn = ext().gqa_launches(self.batch, self.cfg.n_kv_heads, self.local_ctx, sms)
         if self.cp_size > 1 and self.fuse_oproj:
             return self.cfg.n_layers * (attn + 1)
+        if self.w_bits == 4:
+            return self.cfg.n_layers * (attn + (1 if self.cp_size > 1 else 0) + -(-self.batch // 128))
         packed = self.prepack_oproj and self.cfg.hidden % 128 == 0 and self.k_local % 64 == 0
         own = packed or not oproj_mod.library_gemm_pays(self.batch, self.k_local)
         proj = ext().oproj_launches(self.batch, self.cfg.hidden, self.k_local, packed, sms) if own else 0
