@@ -1,5 +1,6 @@
 // Torch bindings of the paged cache's bookkeeping and writes.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -44,16 +45,17 @@ Tables extend_tables(torch::Tensor block_table, torch::Tensor held, torch::Tenso
   check_ints(free_pages, "free_pages", dev, -1);
   check_ints(free_used, "free_used", dev, 1);
   constexpr int64_t kMax = 0x7fffffff;
-  TORCH_CHECK(rows >= 0 && rows <= kMax && block_table.size(1) <= kMax && free_pages.size(0) <= kMax, "rows, max_pages and free pages are counted in 32 bits");
+  TORCH_CHECK(rows >= 0 && rows <= kMax / 2 && block_table.size(1) <= kMax && free_pages.size(0) <= kMax, "rows, max_pages and free pages are counted in 32 bits");
   if (parents) check_ints(*parents, "parents", dev, rows);
+  TORCH_CHECK(!parents || rows <= (1 << 20), "trees have at most 2^20 rows");
   TORCH_CHECK(words >= 0 && words <= helix::kTableMaxWords, "mask_words must be 0 to ", helix::kTableMaxWords);
   TORCH_CHECK(page_size >= 1 && page_size <= (1 << 20), "page_size must be positive");
   TORCH_CHECK(cp_size >= 1 && cp_rank >= 0 && cp_rank < cp_size, "cp_rank must be in [0, cp_size)");
   TORCH_CHECK(interleave >= 1 && interleave * cp_size <= (1 << 28), "interleave must be positive and interleave * cp_size at most 2^28");
   c10::cuda::CUDAGuard guard(dev);
-  const auto i32 = torch::TensorOptions().dtype(torch::kInt32).device(dev), i64 = i32.dtype(torch::kInt64);
-  torch::Tensor slots = torch::empty({rows}, i64), mask = torch::empty({rows, words}, i64), positions = torch::empty({rows}, i32),
-                seq_lens = torch::empty({B}, i32), draft_lens = torch::empty({B}, i32), missing = torch::empty({1}, i32);
+  const auto i32 = [&](int64_t n) { return torch::Tensor(at::detail::empty_cuda({n}, at::kInt, dev, c10::nullopt)); };
+  const auto i64 = [&](at::IntArrayRef n) { return torch::Tensor(at::detail::empty_cuda(n, at::kLong, dev, c10::nullopt)); };
+  torch::Tensor slots = i64({rows}), mask = i64({rows, words}), positions = i32(rows), seq_lens = i32(B), draft_lens = i32(B), missing = i32(1);
   helix::ExtendTablesParams p{};
   p.block_table = block_table.data_ptr<int32_t>();
   p.bt_stride = block_table.stride(0);
@@ -91,7 +93,7 @@ void append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::T
   TORCH_CHECK(k_cache.size(hd) == heads && k_cache.size(3) == D, "the caches must have the rows' kv heads and head_dim");
   TORCH_CHECK(slots.scalar_type() == at::ScalarType::Long && slots.dim() == 1 && slots.is_contiguous() && slots.size(0) == rows,
               "slots must be a contiguous int64 [rows]");
-  TORCH_CHECK(rows <= 0x7fffffff, "rows are counted in 32 bits");
+  TORCH_CHECK(rows <= 0x3fffffff, "at most 2^30 - 1 rows");
   if (k.numel() == 0 || k_cache.numel() == 0) return;
   TORCH_CHECK(D * es % 16 == 0, "a head's row must be a multiple of 16 bytes");
   for (const torch::Tensor* t : {&k, &v, &k_cache, &v_cache}) {

@@ -34,6 +34,11 @@ struct Seq {
   int held, first, got;    // pages held before, first entry of the free list that is taken, how many are
 };
 
+// tokens that n pages hold, as far as 32 bits count
+__device__ __forceinline__ int tokens_of(const ExtendTablesParams& p, int pages) {
+  return (int)min((long long)pages * p.page_size, 0x7fffffffll);
+}
+
 struct Split {                                   // the ranks' shares of a sequence
   int il, cycle, skip;
   __device__ __forceinline__ int local(int n) const { return n / cycle * il + min(max(n % cycle - skip, 0), il); }
@@ -60,9 +65,9 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
       s.ctx = max(__ldg(p.ctx_lens + b), 0);
       s.row0 = min(max(__ldg(p.q_start + b), 0), p.rows);
       s.rows = max(min(__ldg(p.q_start + b + 1), p.rows) - s.row0, 0);
-      s.rows = min(s.rows, 0x7fffffff - s.ctx);
+      s.ctx = min(s.ctx, 0x7fffffff - s.rows);
       s.held = min(max(__ldcg(p.held + b), 0), p.max_pages);
-      const int need = (split.local(s.ctx + s.rows) + p.page_size - 1) / p.page_size;
+      const int need = (int)(((unsigned)split.local(s.ctx + s.rows) + p.page_size - 1) / (unsigned)p.page_size);
       want = max(min(need, p.max_pages) - s.held, 0);
       lack = max(need - p.max_pages, 0);
     }
@@ -113,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
         const int mid = (lo + hi) / 2;
         if (s_seq[mid].row0 <= row) lo = mid; else hi = mid;
       }
-      if (p.B == 0 || row >= last || row < s_seq[lo].row0) {
+      if (p.B == 0 || row < s_seq[lo].row0 || row - s_seq[lo].row0 >= s_seq[lo].rows) {
         p.slots[row] = -1;
         p.positions[row] = 0;
         for (int w = 0; w < p.words; ++w) p.mask[(int64_t)row * p.words + w] = 0;
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
       const int pos = s.ctx + row - s.row0;
       place(s, lo, row, pos);
       p.positions[row] = pos;
-      const int seen = min(split.local(pos + 1), (s.held + s.got) * p.page_size) - split.local(s.ctx);
+      const int seen = min(split.local(pos + 1), tokens_of(p, s.held + s.got)) - split.local(s.ctx);
       for (int w = 0; w < p.words; ++w) {
         const int n = min(max(seen - 64 * w, 0), 64);
         p.mask[(int64_t)row * p.words + w] = n == 64 ? ~0ull : (1ull << n) - 1;
@@ -136,11 +141,20 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
       __syncwarp();
       for (int j = lane; j < min(s.rows, kStagedNodes); j += 32) s_parent[warp][j] = __ldg(p.parents + s.row0 + j);
       __syncwarp();
-      const int base_local = split.local(s.ctx), room = (s.held + s.got) * p.page_size;
-      for (int j = lane; j < s.rows; j += 32) {
+      const int base_local = split.local(s.ctx), room = tokens_of(p, s.held + s.got);
+      for (int j0 = 0; j0 < s.rows; j0 += 32) {
+        const int j = min(j0 + lane, s.rows - 1);         // (lanes behind the end repeat the last node)
         uint64_t words[kTableMaxWords] = {0, 0, 0, 0};
         int depth = 0;
         for (int up = j;;) {
+          if (up < j0 && j0 >= kStagedNodes) {            // a far walk goes on where this warp has been: at most 32 steps
+            const int64_t row = s.row0 + up;
+            depth += __ldcg(p.positions + row) - s.ctx;
+#pragma unroll
+            for (int w = 0; w < kTableMaxWords; ++w)
+              if (w < p.words) words[w] |= __ldcg(reinterpret_cast<const unsigned long long*>(p.mask) + row * p.words + w);
+            break;
+          }
           const int pos = s.ctx + up;
           const int at = split.local(pos), bit = at - base_local;
           if (split.mine(pos) && at < room) {
@@ -157,6 +171,7 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
         place(s, b, row, s.ctx + j);
         p.positions[row] = s.ctx + depth;
         for (int w = 0; w < p.words; ++w) p.mask[(int64_t)row * p.words + w] = words[w];
+        __syncwarp();
       }
     }
     const int first = p.B > 0 ? s_seq[0].row0 : p.rows;
@@ -175,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
     const Seq s = s_seq[b];
     for (int i = lane; i < s.got; i += 32) p.block_table[b * p.bt_stride + s.held + i] = __ldg(p.free_pages + s.first + i);
     if (lane == 0) {
-      const int room = (s.held + s.got) * p.page_size, len = min(split.local(s.ctx + s.rows), room);
+      const int len = min(split.local(s.ctx + s.rows), tokens_of(p, s.held + s.got));
       p.held[b] = s.held + s.got;
       p.seq_lens[b] = len;
       p.draft_lens[b] = max(len - split.local(s.ctx), 0);
@@ -219,7 +234,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < kRowsAhead; ++i)
         if (slot[i] >= 0 && slot[i] < p.n_slots) {
-          const int64_t page = slot[i] / p.page_size;
+          // (64-bit divisions are some 100 instructions, which only slots behind 2^32 need)
+          const int64_t page = slot[i] >> 32 ? slot[i] / p.page_size : (uint32_t)slot[i] / (uint32_t)p.page_size;
           *reinterpret_cast<uint4*>(dst + page * sp + (slot[i] - page * p.page_size) * st) = x[i];
         }
     }
@@ -267,7 +283,7 @@ cudaError_t launch_append_kv(const AppendKvParams& p, bool pdl, cudaStream_t str
   if (p.head_bytes <= 0 || p.head_bytes % 16 != 0 || p.page_size <= 0) return cudaErrorInvalidValue;
   const int per_row = 2 * p.heads * (p.head_bytes / 16);
   const int x = std::min((per_row + 31) / 32 * 32, kAppendThreads), y = std::max(kAppendThreads / x, 1);
-  const int64_t blocks = std::min<int64_t>((p.rows + y - 1) / y, 148 * 8);
+  const int64_t blocks = std::min<int64_t>(((int64_t)p.rows + y - 1) / y, 148 * 8);
   cudaLaunchConfig_t cfg = config(dim3((unsigned)blocks), dim3(x, y), 0, stream);
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -80,6 +80,7 @@ class HelixDecodeStack:
             raise ValueError("w_bits must be 4 or 16")
         self.w_bits = w_bits
         self.draft_tokens = draft_tokens
+        self.plan: Optional[paged.TablePlan] = None
         spare = batch * ((draft_tokens + cfg.page_size - 1) // cfg.page_size + 1) if draft_tokens else 0
         self.n_pages = batch * pages_per_seq + spare
         # pages of a sequence are scattered over the pool, as a paged allocator would leave them
@@ -172,12 +173,13 @@ class HelixDecodeStack:
         """One pass over drafted tokens: ``q_all [L, rows, Hq, D]``, ``k_all`` / ``v_all [L, rows, Hkv, D]``, rows ``q_start[b]`` to
         ``q_start[b + 1]`` are sequence ``b``'s, ``parents [rows]`` their tree (``None``: chains); see :func:`ops.paged.extend_tables`.
         Returns ``y [L, rows, hidden]`` (this rank's partial sums).  Committed lengths stay as they are: the next call overwrites
-        the drafted tokens, unless :meth:`commit` keeps some.  No host synchronisation, so the step can be captured."""
+        the drafted tokens, unless :meth:`commit` keeps some.  No host synchronisation, so the step can be captured.  ``plan`` holds
+        the step's places; where its ``missing`` is not 0 the stack has outgrown ``draft_tokens``, and its last tokens are nowhere."""
         if not self.draft_tokens:
             raise RuntimeError("this stack was made without draft_tokens")
         rows = q_all.shape[1]
         words = min((self.draft_tokens + 63) // 64, 4)
-        plan = self._extend(q_start, rows, parents, words)
+        plan = self.plan = self._extend(q_start, rows, parents, words)
         ys = []
         for l in range(self.cfg.n_layers):
             paged.append_kv(k_all[l], v_all[l], self.k_cache[l], self.v_cache[l], plan.slots)
@@ -193,7 +195,7 @@ class HelixDecodeStack:
         says which of them belong to which sequence.  A path through a tree becomes a run of tokens behind the committed ones."""
         if not self.draft_tokens:
             raise RuntimeError("this stack was made without draft_tokens")
-        plan = self._extend(q_start, accepted.numel(), None, 0)
+        plan = self.plan = self._extend(q_start, accepted.numel(), None, 0)
         for l in range(self.cfg.n_layers):
             paged.append_kv(k_all[l][accepted], v_all[l][accepted], self.k_cache[l], self.v_cache[l], plan.slots)
         self.ctx_lens += q_start.diff()

@@ -101,6 +101,25 @@ def test_tables_walk_of_malformed_parents_ends():
     same(run(state, lens, kw, "cuda"), run(state, lens, kw, "cpu"))
 
 
+@pytest.mark.parametrize("words,cp", [(4, 1), (2, 4), (0, 8)])
+def test_a_tree_of_many_nodes(words, cp):
+    """Walks to the root of a long chain go on where the warp has been."""
+    state, lens, kw = make(words, 3, 1500, 40, 16, cp, 1, True, spare=9)
+    kw = dict(kw, mask_words=words)
+    same(run(state, lens, kw, "cuda"), run(state, lens, kw, "cpu"))
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_lengths_at_the_end_of_32_bits(tree):
+    state = dict(block_table=ints([[3, 4, 5], [6, 7, 8]]), held=ints([2, 1]), free_pages=ints([9, 10, 11]), free_used=ints([0]))
+    lens = dict(ctx_lens=ints([2**31 - 3, 20]), q_start=ints([0, 8, 16]))
+    plan, after = run(state, lens, dict(rows=20, page_size=16, parents=ints(np.arange(20) - 1 - 8 * (np.arange(20) >= 8)) if tree else None), "cuda")
+    # the first sequence takes what its table has room for, the second one needs a page
+    assert after["block_table"].tolist() == [[3, 4, 9], [6, 10, 8]] and after["held"].tolist() == [3, 2]
+    assert plan.slots.tolist() == [-1] * 8 + [10 * 16 + 4 + i for i in range(8)] + [-1] * 4
+    assert int(plan.missing) > 0 and plan.seq_lens.tolist() == [48, 28] and plan.draft_lens.tolist() == [0, 8]
+
+
 def test_tables_in_a_graph_carry_their_state():
     """Replays of one captured call see what the replay before them took, as calls one after the other do."""
     state, lens, kw = make(9, 30, 20, 200, 16, 1, 1, True, spare=400)
@@ -136,7 +155,8 @@ def test_tables_refusals():
     for bad in (dict(held=good["held"].long()), dict(held=good["held"][:3]), dict(q_start=good["q_start"][:4]), dict(free_used=good["held"]),
                 dict(ctx_lens=good["ctx_lens"].cpu()), dict(parents=kw["parents"][:-1]), dict(mask_words=5), dict(mask_words=-1),
                 dict(page_size=0), dict(cp_rank=1), dict(cp_size=0), dict(interleave=0), dict(block_table=good["block_table"].t()),
-                dict(rows=-1), dict(free_pages=good["free_pages"].float())):
+                dict(rows=-1), dict(free_pages=good["free_pages"].float()),
+                dict(rows=2**20 + 1, parents=torch.zeros(2**20 + 1, dtype=torch.int32, device="cuda")), dict(rows=2**30)):
         with pytest.raises(RuntimeError):
             call(**bad)
 
@@ -205,3 +225,15 @@ def test_append_refusals():
                  (k[..., ::2], k[..., ::2], kc[..., :64], vc[..., :64], slots), (k[..., :4], k[..., :4], kc[..., :4], vc[..., :4], slots)):
         with pytest.raises(RuntimeError):
             paged.append_kv(*args)
+
+
+def test_append_to_slots_behind_32_bits():
+    """A cache of 2^33 slots whose pages all lie on one another."""
+    one = [torch.zeros(1, 2, 16, 8, dtype=torch.float16, device="cuda") for _ in range(2)]
+    k, v = torch.randn(2, 3, 2, 8, device="cuda").half()
+    slots = torch.tensor([2**32 + 5, 2**33 - 1, 2**33], device="cuda")
+    paged.append_kv(k, v, one[0].expand(2**29, -1, -1, -1), one[1].expand(2**29, -1, -1, -1), slots)
+    for c, x in zip(one, (k, v)):
+        want = torch.zeros_like(c)
+        want[0, :, 5], want[0, :, 15] = x[0], x[1]
+        assert torch.equal(c, want)
