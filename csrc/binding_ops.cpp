@@ -560,9 +560,9 @@ torch::Tensor oproj_int4(torch::Tensor x, torch::Tensor packed, int64_t hidden, 
   torch::Tensor y = torch::empty({tokens, hidden}, x.options());
   if (tokens == 0) return y;
   ScratchUse sc = scratch_for(dev, false, 0, 0, 0);
-  for (int64_t t0 = 0; t0 < tokens; t0 += helix::int4_max_tokens((int)group)) {
+  for (int64_t t0 = 0; t0 < tokens; t0 += helix::kInt4MaxTokens) {
     helix::OprojInt4Params p{};
-    p.tokens = (int)std::min<int64_t>(tokens - t0, helix::int4_max_tokens((int)group));
+    p.tokens = (int)std::min<int64_t>(tokens - t0, helix::kInt4MaxTokens);
     p.x = reinterpret_cast<const uint16_t*>(x.data_ptr()) + t0 * x.stride(0);
     p.x_stride = x.stride(0);
     const uint64_t dims[2] = {(uint64_t)K, (uint64_t)p.tokens}, strides[1] = {(uint64_t)(p.tokens > 1 ? x.stride(0) : K) * 2};

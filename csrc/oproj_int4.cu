@@ -9,12 +9,16 @@
 // holds as B operands for the whole launch, and walks over 16-row tiles, the next tile's weights on their way.
 //
 // More tokens (oproj_int4_kernel) run on tcgen05.  A CTA owns a slab of 128 rows (M of the MMA; tokens are N) and a run of columns.
-//   * Records of the packed weight arrive by bulk copy.  Two teams of eight warps take them in turn, turn nibbles into numbers and put them
-//     into tensor memory as the MMA's A operand, a thread per row and 64 columns.  (In shared memory a record is 32 KB written and 32 KB read
-//     for 8 KB that arrived.  A record is a chain of waits, loads and stores of ~1600 cycles for its team, so one team alone is half as fast.)
-//   * Every group of a record has an accumulator of its own in tensor memory, filled while the team turns its next record into numbers;
-//     then the same warps, a thread per row and half of the tokens, add it, times its scale, to their sums in registers.
-//   * One barrier tells the MMA warp that a record is in place, its x too, and the accumulators read; one that its MMAs are through.
+// It works in rounds of 256 columns, two records of the packed weight, because what a round takes is mostly chains of waits (a barrier that
+// is ready costs 100 to 200 cycles) and latencies, and every role below is one:
+//   * A warp brings the records by bulk copy, one x.  Eight warps turn nibbles into numbers and put them into tensor memory as the MMA's A
+//     operand, a thread per row and 64 columns of a record.  (In shared memory a record is 32 KB written and 32 KB read for 8 KB that arrived.)
+//   * A warp issues the MMAs.  Every group has an accumulator of its own in tensor memory, a ring of them.
+//   * Further warps add each group, times its scale, to their sums in registers: a thread per row and 32 tokens, 64 with more than 64 (of
+//     32 tokens each, 16 warps took issue slots from the others: 100 tokens 32.2 us).
+// 8192 x 8192 in groups of 128, bf16, in a graph: 32 tokens 22.7 us, 64 tokens 24.9, 100 tokens 30.1.  Before, with teams of warps that did
+// both jobs record by record: 24.7, 28.0, 39.0.  A round takes ~1900 cycles with 32 tokens and ~2900 with 128, of which the tensor cores work
+// ~700 and ~1100; with 128 tokens and groups of 64 the two accumulators that fit are handed to and fro every 64 columns, ~900 cycles each.
 //
 // In both the warps or CTAs that share out the columns meet in shared memory, across a cluster by distributed shared memory: no scratch
 // memory, no atomics, one launch, one order of summation.
@@ -38,8 +42,8 @@ namespace {
 using namespace sm100;
 
 constexpr int kRows = 128;
-constexpr int kTeam = 8, kParts = kTeam / 4;     // warps that dequantise; threads that share a row
-constexpr int kOperand = 64;                           // columns of tensor memory of a record's A operand
+constexpr int kTeam = 8;                               // warps that dequantise, a row and 64 columns of a record per thread
+constexpr int kOperand = 128;                          // columns of tensor memory of a round's A operand
 constexpr int kNibbles = 4096;                         // packed bytes of 64 columns
 constexpr int kMaxRecord = 2 * kNibbles + 4 * 384;     // 128 columns in groups of 32, with zero points
 constexpr int kMaxCluster = 8;
@@ -49,19 +53,17 @@ constexpr int kFewSmem = 200 * 1024;
 
 template <int N>
 struct Shape {
-  // With more than 64 tokens the sums take the registers of a second team, and its accumulators the tensor memory.
-  static constexpr int teams = N <= 64 ? 2 : 1, workers = teams * kTeam;
-  static constexpr int mma_warp = workers, threads = (workers + 2) * 32;           // and a warp that loads
-  static constexpr int slots = 2 * teams;              // records between dequantisation and MMA
-  static constexpr int stages = 8;                     // packed records on their way
-  static constexpr int accs = N <= 32 ? 4 : 2;     // groups of a record: more tokens want larger groups (int4_max_tokens)
-  static constexpr int a_col = teams * accs * N;      // tensor memory: accumulators, then operands
-  static_assert(a_col + slots * kOperand <= 512);
+  static constexpr int tokens = N == 128 ? 64 : 32;    // of a thread that sums
+  static constexpr int sum_warps = 4 * N / tokens;
+  static constexpr int mma_warp = kTeam + sum_warps, w_warp = mma_warp + 1, x_warp = mma_warp + 2, threads = (mma_warp + 3) * 32;
+  static constexpr int slots = 2;                      // rounds, and their x, between dequantisation and MMA
+  static constexpr int stages = 4;                     // packed rounds on their way
+  static constexpr int accs = (512 - slots * kOperand) / N;      // groups between MMA and sums
+  static constexpr int a_col = accs * N;               // tensor memory: accumulators, then operands
   static constexpr int x_bytes = N * 128;              // B operand of 64 columns
-  static constexpr int ring = slots * 2 * x_bytes + stages * kMaxRecord;
-  static constexpr int row = N * 4 + 16;               // bytes between rows of sums on their way, up to 168 rows of either team
-  static constexpr int sums = teams * 168 * row;
-  static constexpr int smem = (ring > sums ? ring : sums) + 1024;
+  static constexpr int ring = slots * 4 * x_bytes + stages * 2 * kMaxRecord;
+  static constexpr int row = N * 4 + 16;               // bytes between rows of sums on their way, up to 168 rows
+  static constexpr int smem = (ring > 168 * row ? ring : 168 * row) + 1024;
 };
 
 template <bool BF16>
@@ -89,38 +91,41 @@ __device__ __forceinline__ uint16_t narrow(float x) {
 // N consecutive columns of this warp's lanes
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[N]) {
-  if constexpr (N == 8)
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "r"(taddr));
-  else if constexpr (N == 16) tmem_ld_32x32b_x16(taddr, v);
+  if constexpr (N == 16) tmem_ld_32x32b_x16(taddr, v);
   else tmem_ld_x32(taddr, v);
 }
 
 template <bool BF16, int N>
 __global__ void __launch_bounds__(Shape<N>::threads, 1) oproj_int4_kernel(const __grid_constant__ OprojInt4Params p) {
   using S = Shape<N>;
-  constexpr int NT = N / kParts;                       // tokens of a worker thread
+  constexpr int NT = S::tokens;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t w_full[S::stages], w_free[S::stages], a_full[S::slots], a_free[S::slots], drain;
+  __shared__ __align__(8) uint64_t w_full[S::stages], w_free[S::stages], a_full[S::slots], a_free[S::slots],
+      g_full[S::accs], g_free[S::accs], drain;
   __shared__ uint32_t tmem_slot;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const x_ring = smem;
-  uint8_t* const w_ring = x_ring + S::slots * 2 * S::x_bytes;
+  uint8_t* const w_ring = x_ring + S::slots * 4 * S::x_bytes;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cl = (int)gridDim.y, rank = (int)blockIdx.y, slab = (int)blockIdx.x;          // a cluster is a column of the grid
-  const int all = (p.K + 127) / 128, r0 = (int)((int64_t)all * rank / cl), records = (int)((int64_t)all * (rank + 1) / cl) - r0;
+  const int all = (p.K + 127) / 128, r0 = (int)((int64_t)all * rank / cl), r1 = (int)((int64_t)all * (rank + 1) / cl), rounds = (r1 - r0 + 1) / 2;
+  const int k0 = r0 * 128, k1 = min(r1 * 128, p.K);    // this CTA's columns
   const int gshift = p.group == 32 ? 5 : p.group == 64 ? 6 : 7, group_bytes = p.zeros ? 384 : 256;
-  auto columns = [&](int r) { return min(128, p.K - (r0 + r) * 128); };                   // of a record: 128, or 64 at the end of K
+  const int record_bytes = 128 * 64 + (128 >> gshift) * group_bytes;
+  auto columns = [&](int r) { return min(256, k1 - k0 - r * 256); };                      // of a round: 64 to 256
 
   if (tid == 0) {
     for (int i = 0; i < S::stages; ++i) {
       mbar_init(&w_full[i], 1);
-      mbar_init(&w_free[i], kTeam);
+      mbar_init(&w_free[i], kTeam + S::sum_warps);     // its nibbles and its scales have been read
     }
     for (int i = 0; i < S::slots; ++i) {
       mbar_init(&a_full[i], kTeam + 1);                // and the bytes of x
       mbar_init(&a_free[i], 1);
+    }
+    for (int i = 0; i < S::accs; ++i) {
+      mbar_init(&g_full[i], 1);
+      mbar_init(&g_free[i], S::sum_warps);
     }
     mbar_init(&drain, 1);
     mbar_fence_init();
@@ -134,149 +139,164 @@ __global__ void __launch_bounds__(Shape<N>::threads, 1) oproj_int4_kernel(const 
   tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   const unsigned long long deadline = now_ns() + p.timeout_ns;
+  auto wait = [&](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, deadline)) != 0; };
   bool ok = true;
 
-  float acc[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j] = 0.f;
-  if (warp < S::workers) {
-    // =========================== dequantisation, and the sums ===========================
-    const int row = tid & (kRows - 1), part = tid >> 7 & 1, team = tid >> 8;               // 64 of a record's columns; half of the tokens
-    const int pair = (row & ~15) + (row & 7) * 2 + (row >> 3 & 1);   // of the row among the scales
-    const uint32_t tq = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + team * (S::accs * N) + part * NT;
+  const int row = tid & (kRows - 1);
+  const int part = warp < kTeam ? warp >> 2 : (warp - kTeam) >> 2;   // 64 columns of a record; NT of the tokens
+  const int pair = (row & ~15) + (row & 7) * 2 + (row >> 3 & 1);     // of the row among the scales
+  const uint32_t tq = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  float2 acc[NT / 2];                                  // of the warps that sum
+  if (warp < kTeam) {
+    // =========================== dequantisation ===========================
     // both in registers: with two constants the compiler makes two instructions of (w & mask) | magic
     uint32_t mask, magic;
     asm volatile("mov.u32 %0, 0x000f000f;" : "=r"(mask));
     asm volatile("mov.u32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300 : 0x64006400));
-    // x of record r, into the place that record r - slots has left
-    auto load_x = [&](int r) {
-      if (warp % kTeam != 0 || lane != 0 || r >= records) return;
-      const int sl = r % S::slots, cols = columns(r);
-      mbar_expect_tx(&a_full[sl], cols / 64 * S::x_bytes);
-      for (int c = 0; c < cols; c += 64)
-        tma_load_2d(x_ring + (sl * 2 + c / 64) * S::x_bytes, &p.x_map, &a_full[sl], (r0 + r) * 128 + c, 0);
-    };
-    if (warp % kTeam == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int r = team; r < S::slots; r += S::teams) load_x(r);
-    float s[S::accs], s_last[S::accs];                             // scales of the row's groups, of this record and of the one before
-    int groups = 0;
-    // the groups of record r, whose MMAs are waited for
-    auto add_groups = [&](int r) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&a_free[r % S::slots], (r / S::slots) & 1, deadline));
-      if (!ok) return;
-      tc_fence_after_sync();
+    for (int r = 0; r < rounds; ++r) {
+      const int st = r % S::stages, sl = r % S::slots, cols = columns(r);
+      ok = wait(&w_full[st], r / S::stages);
+      if (!ok) break;
 #pragma unroll
-      for (int i = 0; i < S::accs; ++i) {
-        if (i < groups) {
-          constexpr int kRun = NT < 32 ? NT : 32;
+      for (int j = 0; j < 2; ++j) {
+        const int here = min(cols - 128 * j, 128);     // columns of the record
+        uint32_t a[32];
+        if (part * 64 < here) {
+          const uint8_t* w = w_ring + st * (2 * kMaxRecord) + j * record_bytes;
+          const uint8_t* zeros = w + here * 64 + ((here >> gshift) << 8);
 #pragma unroll
-          for (int c = 0; c < NT; c += kRun) {
-            uint32_t v[kRun];
-            tmem_ld<kRun>(tq + i * N + c, v);
-            tmem_ld_wait();
+          for (int h = 0; h < 2; ++h) {                // of 32 columns
+            const uint4 q = *reinterpret_cast<const uint4*>(w + (row >> 4) * (here * 8) + (part * 2 + h) * 256 + (row & 15) * 16);
+            const uint32_t z = p.zeros ? zeros[((part * 64 + h * 32) >> gshift) * kRows + pair] : 8u;
+            const uint32_t z2 = magic + (z & 0xfu) * 0x00010001u;    // 128 + z, twice
+            const uint32_t words[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-            for (int j = 0; j < kRun; ++j) acc[c + j] += s_last[i] * __uint_as_float(v[j]);
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) a[16 * h + 4 * c + i] = sub2<BF16>(and_or(words[c] >> (4 * i), mask, magic), z2);
           }
         }
-      }
-      tc_fence_before_sync();
-    };
-    int last = -1;                                     // the team's record before
-    for (int r = team; r < records; last = r, r += S::teams) {
-      const int st = r % S::stages, sl = r % S::slots, cols = columns(r);
-      ok = __all_sync(0xffffffffu, mbar_wait(&w_full[st], (r / S::stages) & 1, deadline));
-      if (!ok) break;
-      // (the operand's place is free: the groups of the record that was there have been added up)
-      const uint8_t* w = w_ring + st * kMaxRecord;
-      const uint8_t* scales = w + cols * 64;
-#pragma unroll
-      for (int i = 0; i < S::accs; ++i) {
-        s_last[i] = s[i];
-        s[i] = (i << gshift) < cols ? widen<BF16>(reinterpret_cast<const uint16_t*>(scales)[i * kRows + pair]) : 0.f;
-      }
-      if (part * 64 < cols) {
-        uint32_t a[32];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {                  // of 32 columns
-          const uint4 q = *reinterpret_cast<const uint4*>(w + (row >> 4) * (cols * 8) + (part * 2 + h) * 256 + (row & 15) * 16);
-          const uint32_t z = p.zeros ? scales[((cols >> gshift) << 8) + ((part * 64 + h * 32) >> gshift) * kRows + pair] : 8u;
-          const uint32_t z2 = magic + (z & 0xfu) * 0x00010001u;      // 128 + z, twice
-          const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[16 * h + 4 * c + i] = sub2<BF16>(and_or(words[c] >> (4 * i), mask, magic), z2);
+        if (j == 0 && r >= S::slots) {
+          ok = wait(&a_free[sl], r / S::slots - 1);
+          if (!ok) break;
+          tc_fence_after_sync();
         }
-        tmem_st_x32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + S::a_col + sl * kOperand + part * 32, a);
-        tmem_st_wait();
-        tc_fence_before_sync();
+        if (part * 64 < here) tmem_st_x32(tq + S::a_col + sl * kOperand + 64 * j + 32 * part, a);
       }
-      if (last >= 0) {
-        add_groups(last);
-        if (ok) load_x(last + S::slots);
-      }
-      groups = cols >> gshift;
-      __syncwarp();
       if (!ok) break;
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
       if (lane == 0) {
         mbar_arrive(&a_full[sl]);
         mbar_arrive(&w_free[st]);
       }
     }
+  } else if (warp < S::mma_warp) {
+    // =========================== sums ===========================
 #pragma unroll
-    for (int i = 0; i < S::accs; ++i) s_last[i] = s[i];
-    if (ok && last >= 0) add_groups(last);
+    for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+    for (int r = 0; r < rounds && ok; ++r) {
+      const int st = r % S::stages, cols = columns(r), groups = cols >> gshift;
+      ok = wait(&w_full[st], r / S::stages);
+      if (!ok) break;
+#pragma unroll 1
+      for (int g = 0; g < groups; ++g) {
+        const int n = r * (256 >> gshift) + g, at = n % S::accs;
+        ok = wait(&g_full[at], n / S::accs);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const int j = g << gshift >> 7, here = min(cols - 128 * j, 128);       // record
+        const uint16_t* scales = reinterpret_cast<const uint16_t*>(w_ring + st * (2 * kMaxRecord) + j * record_bytes + here * 64) + pair;
+        const float s = widen<BF16>(scales[(g - (j << 7 >> gshift)) * kRows]);
+        const float2 s2 = make_float2(s, s);
+        constexpr int kRun = NT == 64 ? 16 : NT;         // as registers allow
+#pragma unroll
+        for (int c = 0; c < NT; c += kRun) {
+          uint32_t v[kRun];
+          tmem_ld<kRun>(tq + at * N + part * NT + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < kRun / 2; ++i) acc[c / 2 + i] = fma2(s2, make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), acc[c / 2 + i]);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&g_free[at]);
+      }
+      if (ok && lane == 0) mbar_arrive(&w_free[st]);
+      __syncwarp();
+    }
   } else if (warp == S::mma_warp) {
     // =========================== MMA issue ===========================
     constexpr uint32_t idesc = BF16 ? umma_idesc_bf16(kRows, N) : umma_idesc_bf16(kRows, N) & ~((1u << 7) | (1u << 10));
     const uint64_t d_x = umma_desc_k_sw128(smem_u32(x_ring));
     auto role = [&](auto shift) {
       constexpr int kShift = decltype(shift)::value;
-      for (int r_lane = 0; r_lane < records && ok; ++r_lane) {
+      constexpr int kGroups = 256 >> kShift;
+      for (int r_lane = 0; r_lane < rounds && ok; ++r_lane) {
         // through a shuffle: what is computed from it is then known to be the same in all lanes, which the MMA's operands want to be
         const int r = __shfl_sync(0xffffffffu, r_lane, 0), sl = r % S::slots, cols = columns(r);
-        ok = __all_sync(0xffffffffu, mbar_wait(&a_full[sl], (r / S::slots) & 1, deadline));
+        ok = wait(&a_full[sl], r / S::slots);
         if (!ok) break;
-        tc_fence_after_sync();
-        const uint32_t td = tmem + r % S::teams * (S::accs * N), ta = tmem + S::a_col + sl * kOperand, x_lo = (uint32_t)d_x + (sl * 2 * S::x_bytes >> 4), x_hi = (uint32_t)(d_x >> 32);
-        if (elect_one()) {
+        const uint32_t ta = tmem + S::a_col + sl * kOperand, x_lo = (uint32_t)d_x + (sl * 4 * S::x_bytes >> 4), x_hi = (uint32_t)(d_x >> 32);
 #pragma unroll
-          for (int k = 0; k < 128; k += 16) {
-            if (k == 64 && cols == 64) break;
-            const uint32_t lo = x_lo + ((k / 64 * S::x_bytes + k % 64 * 2) >> 4), d = td + (k >> kShift) * N;
-            if (k % (1 << kShift) == 0) umma_bf16_ts_first(d, ta + k / 2, lo, x_hi, idesc, 0u);
-            else umma_bf16_ts(d, ta + k / 2, lo, x_hi, idesc);
+        for (int g = 0; g < 256; g += 1 << kShift) {
+          if (g >= cols) break;
+          const int i = g >> kShift, n = r * kGroups + i, at = kGroups < S::accs ? n % S::accs : i % S::accs;
+          if (n >= S::accs && !(ok = wait(&g_free[at], n / S::accs - 1))) break;
+          tc_fence_after_sync();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = g; k < g + (1 << kShift); k += 16) {
+              const uint32_t lo = x_lo + ((k / 64 * S::x_bytes + k % 64 * 2) >> 4);
+              if (k == g) umma_bf16_ts_first(tmem + at * N, ta + k / 2, lo, x_hi, idesc, 0u);
+              else umma_bf16_ts(tmem + at * N, ta + k / 2, lo, x_hi, idesc);
+            }
+            umma_commit(&g_full[at]);
           }
-          umma_commit(&a_free[sl]);
+          __syncwarp();
         }
+        if (ok && elect_one()) umma_commit(&a_free[sl]);
         __syncwarp();
       }
     };
     if (gshift == 5) role(std::integral_constant<int, 5>{});
     else if (gshift == 6) role(std::integral_constant<int, 6>{});
     else role(std::integral_constant<int, 7>{});
+    // the last arrivals have to be there before this CTA leaves
+    for (int r = max(rounds - S::slots, 0); r < rounds && ok; ++r) ok = wait(&a_free[r % S::slots], r / S::slots);
     if (!ok) {
       if (elect_one()) umma_commit(&drain);            // nothing of this CTA's may be in flight when it leaves
       mbar_wait(&drain, 0, now_ns() + 10000000ull);
     }
-  } else {
-    // =========================== loads ===========================
-    const int record_bytes = 128 * 64 + (128 >> gshift) * group_bytes;
+  } else if (warp == S::w_warp) {
+    // =========================== weights ===========================
+    // (they do not depend on the kernel before this one)
     const uint8_t* w = p.w + (int64_t)slab * ((int64_t)p.K * 64 + (int64_t)(p.K >> gshift) * group_bytes) + (int64_t)r0 * record_bytes;
-    int w_at = 0;
-    auto load_w = [&]() {
-      const int st = w_at % S::stages, cols = columns(w_at);
-      if (w_at >= S::stages) ok = __all_sync(0xffffffffu, mbar_wait(&w_free[st], (w_at / S::stages - 1) & 1, deadline));
-      if (!ok) return;
+    for (int r = 0; r < rounds; ++r) {
+      const int st = r % S::stages, cols = columns(r);
+      if (r >= S::stages) ok = wait(&w_free[st], r / S::stages - 1);
+      if (!ok) break;
       const uint32_t bytes = cols * 64 + (cols >> gshift) * group_bytes;
       if (lane == 0) {
         mbar_expect_tx(&w_full[st], bytes);
-        bulk_load_1d(w_ring + st * kMaxRecord, w + (int64_t)w_at * record_bytes, bytes, &w_full[st]);
+        bulk_load_1d(w_ring + st * (2 * kMaxRecord), w + (int64_t)r * 2 * record_bytes, bytes, &w_full[st]);
       }
       __syncwarp();
-      ++w_at;
-    };
-    while (w_at < records && ok) load_w();             // weights do not depend on the kernel before this one
+    }
+  } else {
+    // =========================== x ===========================
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int r = 0; r < rounds; ++r) {
+      const int sl = r % S::slots, cols = columns(r);
+      if (r >= S::slots) ok = wait(&a_free[sl], r / S::slots - 1);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(&a_full[sl], cols / 64 * S::x_bytes);
+        for (int c = 0; c < cols; c += 64) tma_load_2d(x_ring + (sl * 4 + c / 64) * S::x_bytes, &p.x_map, &a_full[sl], k0 + r * 256 + c, 0);
+      }
+      __syncwarp();
+    }
   }
   if (!ok && lane == 0) atomicCAS(p.error_flag, 0, (int)kTimeoutMbarrier);
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -293,9 +313,9 @@ __global__ void __launch_bounds__(Shape<N>::threads, 1) oproj_int4_kernel(const 
     tmem_dealloc(tmem, 512);
   }
 
-  // ---- results: thread (team, part, row) holds tokens part * NT ... of its row, the sum over its team's records ------
-  // Rank r finishes rows r * per ... of the slab.  Everybody is through with its rings, so they take the sums: [rank][team][row].
-  const int row = tid & (kRows - 1), part = tid >> 7 & 1, team = tid >> 8, rows_here = min(kRows, p.hidden - slab * kRows);
+  // ---- results: thread (part, row) of the sums holds tokens part * NT ... of its row -------------------------------
+  // Rank r finishes rows r * per ... of the slab.  Everybody is through with its rings, so they take the sums: [rank][row].
+  const int rows_here = min(kRows, p.hidden - slab * kRows);
   const int per = (kRows / 8 + cl - 1) / cl * 8;
   auto meet = [&]() {
     if (cl == 1) {
@@ -307,13 +327,14 @@ __global__ void __launch_bounds__(Shape<N>::threads, 1) oproj_int4_kernel(const 
     }
   };
   meet();
-  if (warp < S::workers) {
-    const uint32_t at = smem_u32(smem) + ((rank * S::teams + team) * per + row % per) * S::row + part * NT * 4;
+  if (warp >= kTeam && warp < S::mma_warp) {
+    const uint32_t at = smem_u32(smem) + (rank * per + row % per) * S::row + part * NT * 4;
     const uint32_t to = cl == 1 ? at : map_to_cta(at, row / per);
 #pragma unroll
     for (int j = 0; j < NT; j += 4) {
-      if (cl == 1) *reinterpret_cast<float4*>(smem + (at - smem_u32(smem)) + j * 4) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-      else st_cluster_f32x4(to + j * 4, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+      const float2 a = acc[j / 2], b = acc[j / 2 + 1];
+      if (cl == 1) *reinterpret_cast<float4*>(smem + (at - smem_u32(smem)) + j * 4) = make_float4(a.x, a.y, b.x, b.y);
+      else st_cluster_f32x4(to + j * 4, a.x, a.y, b.x, b.y);
     }
   }
   meet();
@@ -323,7 +344,7 @@ __global__ void __launch_bounds__(Shape<N>::threads, 1) oproj_int4_kernel(const 
     if (r >= mine) continue;
     const uint8_t* from = smem + r * S::row + n * 4;
     float v = *reinterpret_cast<const float*>(from);
-    for (int c = 1; c < cl * S::teams; ++c) v += *reinterpret_cast<const float*>(from + c * per * S::row);
+    for (int c = 1; c < cl; ++c) v += *reinterpret_cast<const float*>(from + c * per * S::row);
     p.y[n * p.y_stride + slab * kRows + rank * per + r] = narrow<BF16>(v);
   }
 }
@@ -606,11 +627,11 @@ cudaError_t launch_few(OprojInt4Params p, bool pdl, int sm_count, int dev, cudaS
 
 cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStream_t stream) {
   if (p.tokens <= 0 || p.hidden <= 0) return cudaSuccess;
-  if (p.K <= 0 || p.K % 64 != 0 || (p.group != 32 && p.group != 64 && p.group != 128) || p.K % p.group != 0 || p.tokens > int4_max_tokens(p.group))
+  if (p.K <= 0 || p.K % 64 != 0 || (p.group != 32 && p.group != 64 && p.group != 128) || p.K % p.group != 0 || p.tokens > kInt4MaxTokens)
     return cudaErrorInvalidValue;
   int dev = 0;
   cudaGetDevice(&dev);
-  // Measured in graphs, 8192 x 8192: 8 tokens 12.1 us, 16 tokens 16.6 (two launches of eight 24), the other kernel 24.2 from 17 tokens on.  A
+  // Measured in graphs, 8192 x 8192: 8 tokens 12.1 us, 16 tokens 16.6 (two launches of eight 24), the other kernel 22.7 from 17 tokens on.  A
   // wider K than a cluster's warps hold takes the other kernel, too.
   if (p.tokens <= kInt4FewTokens && p.K <= kMaxCluster * kFewWarps * 256) return launch_few(p, pdl, sm_count, dev, stream);
   size_t smem = 0;

@@ -29,7 +29,7 @@ struct OprojInt4Params {
 };
 
 constexpr int kInt4FewTokens = 16;       // up to so many the weights stay in registers
-constexpr int int4_max_tokens(int group) { return group == 32 ? 32 : 128; }     // of one launch: the accumulators of 128 columns have to fit
+constexpr int kInt4MaxTokens = 128;      // of one launch
 constexpr int int4_pad_tokens(int tokens) { return tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128; }
 constexpr size_t int4_slab_bytes(int64_t K, int64_t group, bool zeros) { return (size_t)(K * 64 + K / group * (zeros ? 384 : 256)); }
 cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStream_t stream);

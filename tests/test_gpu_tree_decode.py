@@ -251,6 +251,35 @@ def test_strides_and_views():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("layout,hkv", [("HND", 1), ("HND", 3), ("NHD", 1), ("NHD", 3)])
+def test_caches_whose_pages_and_heads_lie_apart(layout, hkv, page):
+    """Gaps between tokens, heads and pages, one page only, a page that is not there."""
+    for ctx in ([700, 90], [min(page, 90)] * 1):
+        n = len(ctx)
+        s = make(ctx, [5] * n, [5] * n, 4 * hkv, hkv, page, layout, "bf16", seed=page + hkv)
+        want = attention.tree_decode(*s.values(), layout=layout)
+        for pad in ((0, 1, 0, 0), (0, 0, 1, 0), (1, 0, 0, 0), (0, 1, 1, 0), (0, 0, 0, 8)):
+            c = {}
+            for i, name in enumerate(("k_cache", "v_cache")):
+                shape = s[name].shape
+                room = torch.full([a + b for a, b in zip(shape, pad)], float("nan"), dtype=torch.bfloat16, device="cuda")
+                c[name] = room[tuple(slice(0, x) for x in shape)]
+                c[name].copy_(s[name])
+            got = attention.tree_decode(*dict(s, **c).values(), layout=layout)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # pages outside the cache are pages of zeros, and what lies behind the cache in memory is not read
+    s = make([3 * page], [0], [2], hkv, hkv, page, layout, "bf16")
+    for bad in (s["k_cache"].shape[0], 2 ** 28 + 1, 2 ** 31 - 1, -1):
+        t = dict(s, block_table=s["block_table"].clone(), k_cache=torch.cat([s["k_cache"], torch.full_like(s["k_cache"], 1e30)])[:len(s["k_cache"])])
+        t["block_table"][0, 1] = bad
+        zero = dict(s, k_cache=torch.cat([s["k_cache"], torch.zeros_like(s["k_cache"][:1])]), v_cache=torch.cat([s["v_cache"], torch.zeros_like(s["v_cache"][:1])]),
+                    block_table=s["block_table"].clone())
+        zero["block_table"][0, 1] = s["k_cache"].shape[0]
+        got, want = attention.tree_decode(*t.values(), layout=layout), attention.tree_decode(*zero.values(), layout=layout)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_graph_replays_follow_their_inputs():
     s = make([900, 400, 130], [9, 9, 9], [9, 9, 9], 32, 4, 16, "HND", "bf16", seed=4)
     eager = attention.tree_decode(*s.values(), max_seq_len=900, max_q_len=9)
