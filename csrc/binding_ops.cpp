@@ -302,8 +302,15 @@ std::tuple<torch::Tensor, torch::Tensor> tree_decode(torch::Tensor q, torch::Ten
   p.tiles = plan.tiles;
   p.ctas = plan.ctas;
   p.whole = plan.whole;
-  ScratchUse sc = scratch_for(dev, !p.whole, 0, p.whole ? 0 : (int64_t)helix::tree_part_o_floats(p.ctas, p.tiles),
-                              p.whole ? 0 : (int64_t)helix::tree_part_lse_floats(p.ctas, p.tiles));
+  ScratchUse sc = scratch_for(dev, false, 0, 0, 0);
+  // Pieces lie in memory of the call's own: calls on two streams, and graphs that are replayed together, must not share it
+  torch::Tensor parts;
+  if (!p.whole) {
+    const int64_t n = (int64_t)helix::tree_part_o_floats(p.ctas, p.tiles);
+    parts = torch::empty({n + (int64_t)helix::tree_part_lse_floats(p.ctas, p.tiles)}, lse.options());
+    p.part_o = parts.data_ptr<float>();
+    p.part_lse = p.part_o + n;
+  }
   p.q = reinterpret_cast<const uint16_t*>(q.data_ptr());
   p.q_sr = q.stride(0); p.q_sh = q.stride(1);
   p.v = reinterpret_cast<const uint16_t*>(v_cache.data_ptr());
@@ -317,8 +324,6 @@ std::tuple<torch::Tensor, torch::Tensor> tree_decode(torch::Tensor q, torch::Ten
   p.mask_stride = mask.stride(0);
   p.o = reinterpret_cast<uint16_t*>(o.data_ptr());
   p.lse = lse.data_ptr<float>();
-  p.part_o = p.whole ? nullptr : sc.set.part_a.data_ptr<float>();
-  p.part_lse = p.whole ? nullptr : sc.set.part_b.data_ptr<float>();
   p.error_flag = sc.dev.error_flag.data_ptr<int32_t>();
   p.rows = (int)rows; p.B = (int)B; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.page_size = (int)page; p.max_pages = (int)block_table.size(1);
   p.n_pages = (int)pages; p.words = (int)mask.size(1);

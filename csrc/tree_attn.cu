@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
     }
   } else if (warp >= kMmaWarp) {
     // =========================== MMA issue ===========================
-    // rows that no unit covers: those of sequences without a token here, and those behind the last sequence
+    // rows that no unit covers: those of sequences without a token here, and those before the first and behind the last sequence
     if (warp == kMmaWarp) {
       auto clear = [&](int r0, int r1) {
         for (int64_t i = (int64_t)r0 * p.Hq * 16 + lane; i < (int64_t)r1 * p.Hq * 16; i += 32) {
@@ -667,6 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_kernel(const __grid_c
       };
       for (int b = blockIdx.x; b < p.B; b += gridDim.x)
         if (seq_len_of(p, b) == 0) clear(row0_of(p, b), row0_of(p, b + 1));
+      for (int r = blockIdx.x; r < row0_of(p, 0); r += gridDim.x) clear(r, r + 1);
       for (int r = row0_of(p, p.B) + blockIdx.x; r < p.rows; r += gridDim.x) clear(r, r + 1);
     }
     constexpr uint32_t fmt = BF16 ? umma_idesc_bf16(kRows, kTile) : umma_idesc_bf16(kRows, kTile) & ~((1u << 7) | (1u << 10));

@@ -142,6 +142,8 @@ def pack_weight_int4(qweight: torch.Tensor, scales: torch.Tensor, zeros: Optiona
         raise ValueError("pack_weight_int4 needs K % 64 == 0 and scales [hidden, K / group], group 32, 64 or 128")
     if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
         raise ValueError("zeros must be uint8 of the scales' shape")
+    if zeros is not None and int(zeros.max()) > 15:
+        raise ValueError("zeros must be 0 .. 15")
     slabs = -(-hidden // 128)
 
     def in_slabs(t):

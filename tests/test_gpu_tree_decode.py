@@ -280,6 +280,15 @@ def test_caches_whose_pages_and_heads_lie_apart(layout, hkv, page):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_rows_before_the_first_sequence():
+    s = make([90, 40], [4, 4], [4, 4], 16, 2, 16, "HND", "bf16", pad=7)
+    t = {k: torch.cat([torch.randn_like(v[:3]) if v.is_floating_point() else v[:3], v]) if k in ("q", "mask") else v for k, v in s.items()}
+    t["q_start"] = s["q_start"] + 3
+    torch.full((1 << 22,), float("nan"), device="cuda")                     # what fresh memory may hold
+    o, lse = check(t, "HND", "bf16")
+    assert not o[:3].any() and (lse[:3] == -math.inf).all()
+
+
 def test_graph_replays_follow_their_inputs():
     s = make([900, 400, 130], [9, 9, 9], [9, 9, 9], 32, 4, 16, "HND", "bf16", seed=4)
     eager = attention.tree_decode(*s.values(), max_seq_len=900, max_q_len=9)
@@ -298,6 +307,40 @@ def test_graph_replays_follow_their_inputs():
     want, want_lse, a = exact(s, "HND")
     assert ((o.double() - want).abs() <= 2 ** -8 * (a + want.abs()) + 2e-4 * a).all()
     assert not o[20:].any() and (lse[20:] == -math.inf).all()
+
+
+def test_calls_at_once():
+    """Split calls on two streams, and graphs of both replayed together, have each its own scratch."""
+    kw = dict(max_seq_len=6000, max_q_len=20)
+    inputs = [make([6000, 3000], [20, 20], [20, 20], 32, 4, 16, "HND", "bf16", seed=s) for s in (1, 2)]
+    want = [attention.tree_decode(*s.values(), **kw) for s in inputs]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in inputs], [], []
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s, st in zip(inputs, streams):
+            with torch.cuda.stream(st):
+                got.append(attention.tree_decode(*s.values(), **kw))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+    for s, st in zip(inputs, streams):
+        with torch.cuda.stream(st):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                outs.append([attention.tree_decode(*s.values(), **kw) for _ in range(3)])
+            graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        eager = attention.tree_decode(*inputs[0].values(), **kw)
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            for x in o:
+                assert torch.equal(x[0], w[0]) and torch.equal(x[1], w[1])
+        assert torch.equal(eager[0], want[0][0])
 
 
 def test_same_call_same_bits():

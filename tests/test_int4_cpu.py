@@ -60,7 +60,7 @@ def test_quantisation_is_off_by_half_a_step(dtype, zero_points):
 def test_refusals():
     q, s, z = arrays(32, 128, 64, True)
     b = q[:, 0::2] | (q[:, 1::2] << 4)
-    for bad in ((b.int(), s, z), (b, s.float(), z), (b, s[:, :1].repeat(1, 3), z), (b, s, z[:16]), (b, s, z.int()),
+    for bad in ((b.int(), s, z), (b, s.float(), z), (b, s[:, :1].repeat(1, 3), z), (b, s, z[:16]), (b, s, z.int()), (b, s, z + 16),
                 (b[:, :16], s, z), (b[:0], s[:0], None)):
         with pytest.raises(ValueError):
             oproj.pack_weight_int4(*bad)
