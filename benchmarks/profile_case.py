@@ -10,6 +10,9 @@
     python benchmarks/profile_case.py fused_rows  # the same with 64 tokens (slabs of a head group share the rows)
     python benchmarks/profile_case.py streamk   # stream-K o_proj, 8 tokens, K=8192, hidden 8192
     python benchmarks/profile_case.py combine   # stand-alone LSE combine, 8 ranks x 4096 rows x 512
+    python benchmarks/profile_case.py tree      # tree attention, B=8, 16 drafted tokens each, 16K tokens per sequence (537 MB of KV)
+    python benchmarks/profile_case.py tree_wide # the same for one sequence of 64K tokens and 64 drafted ones (268 MB of KV)
+    python benchmarks/profile_case.py int4      # o_proj with 4-bit weights, 100 tokens, K=8192, hidden 8192
 """
 import os
 import sys
@@ -45,6 +48,28 @@ def main():
         x = torch.randn(8, 8192, device="cuda").bfloat16()
         for _ in range(launches):
             oproj(x, w, splits=-1)
+    elif which in ("tree", "tree_wide"):
+        from helix_a2a_b200.ops import attention, paged
+        B, ctx, drafts = (8, 16384, 16) if which == "tree" else (1, 65536, 64)
+        pages, words = ctx // 16 + drafts // 16, (drafts + 63) // 64
+
+        def i32(*v):
+            return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+        table = torch.randperm(B * pages).int().view(B, -1).cuda()
+        plan = paged.extend_tables(table, i32(*[pages] * B), i32(), i32(0), i32(*[ctx] * B), i32(*range(0, B * drafts + 1, drafts)),
+                                   rows=B * drafts, page_size=16, mask_words=words)
+        kc, vc = (torch.randn(B * pages, 8, 16, 128, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        q = torch.randn(B * drafts, 64, 128, device="cuda", dtype=torch.bfloat16)
+        for _ in range(launches):
+            attention.tree_decode(q, kc, vc, table, plan.seq_lens, i32(*range(0, B * drafts + 1, drafts)), plan.draft_lens, plan.mask,
+                                  max_seq_len=ctx + drafts, max_q_len=drafts)
+    elif which == "int4":
+        from helix_a2a_b200.ops import oproj
+        w = oproj.quantize_weight_int4((torch.randn(8192, 8192, device="cuda") * 0.02).bfloat16())
+        x = torch.randn(100, 8192, device="cuda").bfloat16()
+        for _ in range(launches):
+            oproj.oproj(x, w)
     elif which == "combine":
         import helix_a2a_b200 as helix
         o = torch.randn(8, 32, 128, 512, device="cuda").bfloat16()
