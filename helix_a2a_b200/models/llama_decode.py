@@ -171,7 +171,8 @@ class HelixDecodeStack:
     def verify_step(self, q_all: torch.Tensor, k_all: torch.Tensor, v_all: torch.Tensor, q_start: torch.Tensor,
                     parents: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One pass over drafted tokens: ``q_all [L, rows, Hq, D]``, ``k_all`` / ``v_all [L, rows, Hkv, D]``, rows ``q_start[b]`` to
-        ``q_start[b + 1]`` are sequence ``b``'s, ``parents [rows]`` their tree (``None``: chains); see :func:`ops.paged.extend_tables`.
+        ``q_start[b + 1]`` are sequence ``b``'s, ``parents [rows]`` their tree (``None``: chains), at most 256 of a sequence on a
+        rank; see :func:`ops.paged.extend_tables`.
         Returns ``y [L, rows, hidden]`` (this rank's partial sums).  Committed lengths stay as they are: the next call overwrites
         the drafted tokens, unless :meth:`commit` keeps some.  No host synchronisation, so the step can be captured.  ``plan`` holds
         the step's places; where its ``missing`` is not 0 the stack has outgrown ``draft_tokens``, and its last tokens are nowhere."""
@@ -278,7 +279,7 @@ class HelixDecodeStack:
         """Kernels of this library that one step launches (a split attention or o_proj call is two); counted for a GPU of 148
         SMs where the stack is not on one."""
         sms = torch.cuda.get_device_properties(self.device).multi_processor_count if self.device.type == "cuda" else 148
-        attn = ext().gqa_launches(self.batch, self.cfg.n_kv_heads, self.local_ctx, sms)
+        attn = ext().gqa_launches(self.batch, self.cfg.n_kv_heads, self.max_local, sms)
         if self.cp_size > 1 and self.fuse_oproj:
             return self.cfg.n_layers * (attn + 1)
         if self.w_bits == 4:
