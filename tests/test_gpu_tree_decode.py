@@ -343,6 +343,17 @@ def test_calls_at_once():
         assert torch.equal(eager[0], want[0][0])
 
 
+@pytest.mark.parametrize("lens,counts,hq,hkv", [([9000], [64], 64, 8), ([5000, 3000, 700], [40, 40, 40], 64, 8), ([4000, 4100], [33, 60], 64, 8), ([6000], [150], 32, 4),
+                                                ([3000, 0, 2000], [50, 9, 50], 96, 4), ([2500], [256], 64, 1), ([20000], [37], 56, 8),
+                                                ([1000] * 150, [40] * 150, 8, 1)])
+def test_groups_of_rows_side_by_side(lens, counts, hq, hkv):
+    """Sequences with several groups of 256 rows each: as many for all of them, or not, and numbers that do not divide the CTAs."""
+    drafts = [min(n, c) for n, c in zip(lens, counts)]
+    s = make(lens, drafts, counts, hq, hkv, 16, "HND", "bf16", words=4, pad=3, seed=len(lens))
+    check(s, "HND", "bf16", max_seq_len=max(lens), max_q_len=max(counts))
+    check(s, "HND", "bf16")
+
+
 def test_same_call_same_bits():
     s = make([5000, 17, 2600], [30, 10, 30], [30, 10, 30], 64, 8, 16, "HND", "bf16", seed=6)
     first = attention.tree_decode(*s.values(), max_seq_len=5000, max_q_len=30)
