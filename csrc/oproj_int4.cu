@@ -641,14 +641,16 @@ cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStr
   Resident r;
   const cudaError_t e = resident((const void*)fn, dev, threads, smem, smem, sm_count, &r);
   if (e != cudaSuccess) return e;
-  // As many CTAs per slab as make the launch shortest: rounds of resident clusters times the records of a CTA, and about three records'
-  // time for a CTA's start, the exchange and the end.
+  // As many CTAs per slab as make the launch shortest: rounds of resident clusters times the records of a CTA, and about ten records'
+  // time for a CTA's start, the exchange and the end.  Measured with 100 tokens, clusters of 1 / 2 / 3 / 4 CTAs (74 clusters of two fit, 33 of
+  // four): 8192 x 8192 45.6 / 29.5 / 46.1 / 39.5 us, 4096 x 4096 26.9 / 19.0 / 16.9 / 15.1, 28672 x 8192 91.0 / 110.7 / 125.1 / 132.6; the least is chosen
+  // at all nine shapes that were tried, with 32 and 64 tokens too.
   const int slabs = (p.hidden + kRows - 1) / kRows, records = (p.K + 127) / 128;
   int best = 1;
   int64_t cost = INT64_MAX;
   for (int cl = 1; cl <= std::min(kMaxCluster, records); ++cl) {
     if (r.clusters[cl] < 1) continue;
-    const int64_t c = (int64_t)((slabs + r.clusters[cl] - 1) / r.clusters[cl]) * ((records + cl - 1) / cl + 3);
+    const int64_t c = (int64_t)((slabs + r.clusters[cl] - 1) / r.clusters[cl]) * ((records + cl - 1) / cl + 10);
     if (c < cost) {
       cost = c;
       best = cl;
