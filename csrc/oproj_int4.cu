@@ -16,7 +16,7 @@
 //   * A warp issues the MMAs.  Every group has an accumulator of its own in tensor memory, a ring of them.
 //   * Further warps add each group, times its scale, to their sums in registers: a thread per row and 32 tokens, 64 with more than 64 (of
 //     32 tokens each, 16 warps took issue slots from the others: 100 tokens 32.2 us).
-// 8192 x 8192 in groups of 128, bf16, in a graph: 32 tokens 22.7 us, 64 tokens 24.9, 100 tokens 30.1.  Before, with teams of warps that did
+// 8192 x 8192 in groups of 128, bf16, in a graph: 32 tokens 21.6 us, 64 tokens 23.7, 100 tokens 27.5.  Before, with teams of warps that did
 // both jobs record by record: 24.7, 28.0, 39.0.  A round takes ~1900 cycles with 32 tokens and ~2900 with 128, of which the tensor cores work
 // ~700 and ~1100; with 128 tokens and groups of 64 the two accumulators that fit are handed to and fro every 64 columns, ~900 cycles each.
 //
@@ -328,24 +328,33 @@ __global__ void __launch_bounds__(Shape<N>::threads, 1) oproj_int4_kernel(const 
   };
   meet();
   if (warp >= kTeam && warp < S::mma_warp) {
-    const uint32_t at = smem_u32(smem) + (rank * per + row % per) * S::row + part * NT * 4;
-    const uint32_t to = cl == 1 ? at : map_to_cta(at, row / per);
+    uint8_t* const at = smem + (rank * per + row % per) * S::row + part * NT * 4;
+    const int owner = row / per;
+    const uint32_t to = map_to_cta(smem_u32(at), owner);
 #pragma unroll
     for (int j = 0; j < NT; j += 4) {
       const float2 a = acc[j / 2], b = acc[j / 2 + 1];
-      if (cl == 1) *reinterpret_cast<float4*>(smem + (at - smem_u32(smem)) + j * 4) = make_float4(a.x, a.y, b.x, b.y);
+      if (owner == rank) *reinterpret_cast<float4*>(at + j * 4) = make_float4(a.x, a.y, b.x, b.y);
       else st_cluster_f32x4(to + j * 4, a.x, a.y, b.x, b.y);
     }
   }
   meet();
-  const int mine = max(min(per, rows_here - rank * per), 0);
-  for (int e = tid; e < per * p.tokens; e += S::threads) {
-    const int n = e / per, r = e % per;
+  // a row and four tokens at a time: 16-byte reads of rows that lie 16 bytes past a multiple of 128 apart meet no bank twice
+  const int mine = max(min(per, rows_here - rank * per), 0), quads = (p.tokens + 3) / 4;
+  for (int e = tid; e < per * quads; e += S::threads) {
+    const int n = e / per * 4, r = e % per;
     if (r >= mine) continue;
     const uint8_t* from = smem + r * S::row + n * 4;
-    float v = *reinterpret_cast<const float*>(from);
-    for (int c = 1; c < cl; ++c) v += *reinterpret_cast<const float*>(from + c * per * S::row);
-    p.y[n * p.y_stride + slab * kRows + rank * per + r] = narrow<BF16>(v);
+    float4 v = *reinterpret_cast<const float4*>(from);
+    for (int c = 1; c < cl; ++c) {
+      const float4 w = *reinterpret_cast<const float4*>(from + c * per * S::row);
+      v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+    }
+    const float o[4] = {v.x, v.y, v.z, v.w};
+    uint16_t* y = p.y + (int64_t)n * p.y_stride + slab * kRows + rank * per + r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.tokens) y[i * p.y_stride] = narrow<BF16>(o[i]);
   }
 }
 
@@ -631,7 +640,7 @@ cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStr
     return cudaErrorInvalidValue;
   int dev = 0;
   cudaGetDevice(&dev);
-  // Measured in graphs, 8192 x 8192: 8 tokens 12.1 us, 16 tokens 16.6 (two launches of eight 24), the other kernel 22.7 from 17 tokens on.  A
+  // Measured in graphs, 8192 x 8192: 8 tokens 12.1 us, 16 tokens 16.6 (two launches of eight 24), the other kernel 21.2 from 17 tokens on.  A
   // wider K than a cluster's warps hold takes the other kernel, too.
   if (p.tokens <= kInt4FewTokens && p.K <= kMaxCluster * kFewWarps * 256) return launch_few(p, pdl, sm_count, dev, stream);
   size_t smem = 0;
@@ -643,7 +652,7 @@ cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStr
   if (e != cudaSuccess) return e;
   // As many CTAs per slab as make the launch shortest: rounds of resident clusters times the records of a CTA, and about ten records'
   // time for a CTA's start, the exchange and the end.  Measured with 100 tokens, clusters of 1 / 2 / 3 / 4 CTAs (74 clusters of two fit, 33 of
-  // four): 8192 x 8192 45.6 / 29.5 / 46.1 / 39.5 us, 4096 x 4096 26.9 / 19.0 / 16.9 / 15.1, 28672 x 8192 91.0 / 110.7 / 125.1 / 132.6; the least is chosen
+  // four, the output then 2 us slower): 8192 x 8192 45.6 / 29.5 / 46.1 / 39.5 us, 4096 x 4096 26.9 / 19.0 / 16.9 / 15.1, 28672 x 8192 91.0 / 110.7 / 125.1 / 132.6; the least is chosen
   // at all nine shapes that were tried, with 32 and 64 tokens too.
   const int slabs = (p.hidden + kRows - 1) / kRows, records = (p.K + 127) / 128;
   int best = 1;
