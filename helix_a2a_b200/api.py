@@ -173,11 +173,11 @@ def alltoall_combine_oproj(attn_out: torch.Tensor, lse: torch.Tensor, w_o, works
     sum).  GEMM CTAs request their weights first, then receive and combine the rows of their own heads straight
     into the tensor-core operand in shared memory; the combined activation never goes through global memory.
     On CPU tensors, or when the shape does not fit (more than 64 tokens, a head wider than 512 dims, more GEMM
-    CTAs than SMs), the exchange and the GEMM run as two launches.
+    CTAs than SMs), or ``w_o`` is an ``ops.oproj.Int4OprojWeight``, the exchange and the GEMM run as two launches.
     """
     from .ops import oproj as _oproj
     B = attn_out.shape[0]
-    if isinstance(workspace, CpuWorkspace) or not attn_out.is_cuda or cp_size == 1:
+    if isinstance(workspace, CpuWorkspace) or not attn_out.is_cuda or cp_size == 1 or isinstance(w_o, _oproj.Int4OprojWeight):
         x = alltoall_combine(attn_out, lse, workspace, cp_rank, cp_size, base2=base2) if cp_size > 1 else attn_out
         return _oproj.oproj(x.reshape(B, -1), w_o)
     from .ops._ext import ops

@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from helix_a2a_b200 import lse_combine
+from helix_a2a_b200 import api, lse_combine
 from helix_a2a_b200.models.llama_decode import HelixDecodeStack, LlamaDecodeConfig
 from helix_a2a_b200.ops import attention, oproj, paged
 
@@ -143,6 +143,16 @@ def test_shards_of_ranks_combine_to_the_whole(device, cp, il):
         o, a = plain(q[r0:r0 + c], torch.cat([old[b][0], k[r0:r0 + c]]), torch.cat([old[b][1], v[r0:r0 + c]]), seen)
         # the parts' roundings are weighted like the parts, the combination is rounded once more
         assert ((got[r0:r0 + c] - o).abs() <= 2 * E * (a + o.abs()) + 4e-4 * a).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_exchange_and_o_proj_with_four_bits(device, monkeypatch):
+    """The call that would be one kernel takes 4-bit weights too, as two."""
+    o, lse = torch.randn(5, 8, 128).bfloat16().to(device), torch.randn(5, 8).to(device)
+    w = oproj.quantize_weight_int4(torch.randn(256, 512).bfloat16().to(device))
+    monkeypatch.setattr(api, "alltoall_combine", lambda o, lse, ws, rank, size, base2=False: o[:, 4 * rank:4 * rank + 4])
+    got = api.alltoall_combine_oproj(o, lse, w, None, 1, 2)
+    assert torch.equal(got, oproj.oproj(o[:, 4:].reshape(5, 512), w))
 
 
 @pytest.mark.gpu
