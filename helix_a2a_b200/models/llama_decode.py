@@ -88,7 +88,6 @@ class HelixDecodeStack:
         owned = perm[:batch * pages_per_seq].view(batch, pages_per_seq)
         self.block_table = torch.nn.functional.pad(owned, (0, spare // batch if spare else 0)).to(self.device)
         self.seq_lens = torch.full((batch,), local_ctx, dtype=torch.int32, device=self.device)
-        self.max_local = self.block_table.shape[1] * cfg.page_size if draft_tokens else local_ctx
         # state of ops.paged.extend_tables: the pages each sequence holds, the free ones, committed tokens over all ranks
         self.held = torch.full((batch,), pages_per_seq, dtype=torch.int32, device=self.device)
         self.free_pages = perm[batch * pages_per_seq:].to(self.device)
@@ -121,6 +120,11 @@ class HelixDecodeStack:
         self._static_y = None
 
     # ---- one layer / one step --------------------------------------------------------------------
+    @property
+    def max_local(self) -> int:
+        """Most tokens that a sequence can have on this rank."""
+        return self.block_table.shape[1] * self.cfg.page_size if self.draft_tokens else self.local_ctx
+
     def layer(self, l: int, q: torch.Tensor) -> torch.Tensor:
         with nvtx_range(f"layer{l}.attention"):
             o, lse = attention.gqa_decode(q, self.k_cache[l], self.v_cache[l], self.block_table, self.seq_lens,
