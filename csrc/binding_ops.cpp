@@ -740,6 +740,12 @@ int oproj_launches(int tokens, int hidden, int K, bool packed, int sm_count) {
   return n;
 }
 
+// (cluster, warps, clusters in the grid, batch, batches, inboxes, bytes of shared memory)
+std::tuple<int, int, int, int, int, int, int64_t> int4_few_plan(int tokens, int hidden, int K, int resident) {
+  const helix::Int4FewPlan p = helix::int4_few_plan(tokens, hidden, K, resident);
+  return {p.cl, p.warps, p.columns, p.batch, p.batches, p.inboxes, (int64_t)p.bytes};
+}
+
 int64_t read_error_flag(torch::Tensor like) {
   ScratchUse sc = scratch_for(like.device(), false, 1, 0, 0);
   return sc.dev.error_flag.item<int>();
@@ -788,5 +794,6 @@ void bind_compute(pybind11::module_& m) {
   m.def("oproj_pick_splits_few", &helix::oproj_pick_splits_few);
   m.def("gqa_launches", &gqa_launches);
   m.def("oproj_launches", &oproj_launches);
+  m.def("int4_few_plan", &int4_few_plan);
   m.def("fused_oproj_fits", &fused_oproj_fits);
 }

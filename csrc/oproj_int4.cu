@@ -380,7 +380,7 @@ template <bool BF16, int NT, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) oproj_int4_few_kernel(const __grid_constant__ OprojInt4Params p) {
   constexpr int kGroups = 256 / GROUP;                 // of a warp's columns
   constexpr int kSum = 8 * NT * kRow;                  // sums of one row tile
-  extern __shared__ __align__(128) uint8_t smem[];     // [warps][batch] sums, [2][ranks][batch] of other CTAs
+  extern __shared__ __align__(128) uint8_t smem[];     // [warps][batch] sums, [inboxes][ranks][batch] of other CTAs
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int warps = blockDim.x >> 5, cl = (int)gridDim.y, rank = (int)blockIdx.y;        // a cluster is a column of the grid
   const int col0 = (rank * warps + warp) * 256, blocks = min(max(p.K - col0, 0), 256) / 32;        // of 32 columns
@@ -608,31 +608,50 @@ cudaError_t resident(const void* fn, int dev, int threads, size_t smem, size_t m
 }
 
 cudaError_t launch_few(OprojInt4Params p, bool pdl, int sm_count, int dev, cudaStream_t stream) {
-  const int slices = (p.K + 255) / 256, nt = (p.tokens + 7) / 8, tiles = (p.hidden + 15) / 16;
+  const int nt = (p.tokens + 7) / 8, tiles = (p.hidden + 15) / 16;
   const bool zeros = p.zeros != 0;
   const Fn fn = p.is_bf16 ? (nt == 1 ? pick_few<true, 1>(p.group, zeros) : pick_few<true, 2>(p.group, zeros))
                           : (nt == 1 ? pick_few<false, 1>(p.group, zeros) : pick_few<false, 2>(p.group, zeros));
-  int cl = 1;
-  while (slices > cl * kFewWarps) cl *= 2;
-  const int warps = (slices + cl - 1) / cl;
-  // Row tiles per CTA as if as many CTAs as have registers fitted on an SM; no more room for sums than that takes.
-  const int guess = std::max(sm_count * (kFewWarps / warps) / cl, 1), per = (tiles + guess - 1) / guess;
-  auto bytes = [&](int batch) {
-    const int inboxes = cl == 1 ? 0 : per <= batch ? cl : 2 * cl;
-    return (size_t)batch * 8 * nt * (warps * kRow + inboxes * 16) * sizeof(float);
-  };
-  p.batch = std::min(per, 8);
-  while (p.batch > 1 && bytes(p.batch) > (size_t)kFewSmem) --p.batch;
-  Resident r;
-  const cudaError_t e = resident((const void*)fn, dev, warps * 32, bytes(p.batch), kFewSmem, sm_count, &r);
+  Int4FewPlan plan = int4_few_plan(p.tokens, p.hidden, p.K, sm_count);
+  Resident r{};
+  cudaError_t e;
+  if (plan.cl == 1) {
+    // Row tiles per CTA as if as many CTAs as have registers fitted on an SM; no more room for sums than that takes.  Without other CTAs'
+    // sums any number of batches is right, so the grid may turn out another one.
+    plan = int4_few_plan(p.tokens, p.hidden, p.K, sm_count * (kFewWarps / plan.warps));
+    e = resident((const void*)fn, dev, plan.warps * 32, plan.bytes, kFewSmem, sm_count, &r);
+    plan.columns = std::min(tiles, r.clusters[1]);
+  } else {
+    // The plan has to be that of the grid: a second batch writes to a second set of inboxes.  (A CTA of nine or more warps has an SM to
+    // itself, so it costs nothing to ask with the largest size.)
+    e = resident((const void*)fn, dev, plan.warps * 32, kFewSmem, kFewSmem, sm_count, &r);
+    if (e == cudaSuccess && r.clusters[plan.cl] > 0) plan = int4_few_plan(p.tokens, p.hidden, p.K, r.clusters[plan.cl]);
+  }
   if (e != cudaSuccess) return e;
-  if (r.clusters[cl] < 1) return cudaErrorInvalidConfiguration;
+  if (r.clusters[plan.cl] < 1 || plan.bytes > (size_t)kFewSmem) return cudaErrorInvalidConfiguration;
+  p.batch = plan.batch;
   cudaLaunchAttribute attrs[2];
-  const cudaLaunchConfig_t cfg = config(std::min(tiles, r.clusters[cl]), cl, warps * 32, bytes(p.batch), pdl, stream, attrs);
+  const cudaLaunchConfig_t cfg = config(plan.columns, plan.cl, plan.warps * 32, plan.bytes, pdl, stream, attrs);
   return cudaLaunchKernelEx(&cfg, fn, p);
 }
 
 }  // namespace
+
+Int4FewPlan int4_few_plan(int tokens, int hidden, int K, int resident) {
+  const int slices = (K + 255) / 256, nt = (tokens + 7) / 8, tiles = (hidden + 15) / 16;
+  Int4FewPlan plan{};
+  plan.cl = 1;
+  while (slices > plan.cl * kFewWarps) plan.cl *= 2;
+  plan.warps = (slices + plan.cl - 1) / plan.cl;
+  plan.columns = std::max(std::min(tiles, resident), 1);
+  const int per = (tiles + plan.columns - 1) / plan.columns;
+  for (plan.batch = std::min(per, 8);; --plan.batch) {
+    plan.batches = (per + plan.batch - 1) / plan.batch;
+    plan.inboxes = plan.cl == 1 ? 0 : std::min(plan.batches, 2);
+    plan.bytes = (size_t)plan.batch * 8 * nt * (plan.warps * kRow + plan.inboxes * plan.cl * 16) * sizeof(float);
+    if (plan.batch == 1 || plan.bytes <= (size_t)kFewSmem) return plan;
+  }
+}
 
 cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStream_t stream) {
   if (p.tokens <= 0 || p.hidden <= 0) return cudaSuccess;

@@ -31,6 +31,17 @@ struct OprojInt4Params {
 constexpr int kInt4FewTokens = 16;       // up to so many the weights stay in registers
 constexpr int kInt4MaxTokens = 128;      // of one launch
 constexpr int int4_pad_tokens(int tokens) { return tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128; }
+// How up to kInt4FewTokens tokens are divided: clusters of `cl` CTAs side by side cover K, a warp 256 columns, and cluster i takes the 16-row
+// tiles i, i + columns, ...
+struct Int4FewPlan {
+  int cl, warps, columns;
+  int batch;        // row tiles whose sums a CTA keeps before it adds them up and sends them on
+  int batches;      // of the cluster with the most tiles
+  int inboxes;      // sets of other CTAs' sums in shared memory: the batches take turns at two, a single one needs only its own
+  size_t bytes;     // of shared memory
+};
+// for a grid of at most `resident` clusters
+Int4FewPlan int4_few_plan(int tokens, int hidden, int K, int resident);
 constexpr size_t int4_slab_bytes(int64_t K, int64_t group, bool zeros) { return (size_t)(K * 64 + K / group * (zeros ? 384 : 256)); }
 cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStream_t stream);
 
