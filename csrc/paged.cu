@@ -48,7 +48,8 @@ struct Split {                                   // the ranks' shares of a seque
 
 __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_constant__ ExtendTablesParams p) {
   extern __shared__ Seq s_seq[];
-  __shared__ int s_warp[kWarps], s_want[kWarps], s_parent[kWarps][kStagedNodes];
+  __shared__ long long s_warp[kWarps], s_want[kWarps];
+  __shared__ int s_parent[kWarps][kStagedNodes];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ctas = gridDim.x, cta = blockIdx.x;
   const Split split{p.interleave, p.interleave * p.cp_size, p.interleave * p.cp_rank};
@@ -57,7 +58,8 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
 
   // ---- all sequences: lengths, and the prefix sum of the pages they take ---------------------------------
   const int used = max(__ldcg(p.free_used), 0);
-  int base = 0, short_of = 0;                    // taken (asked for) by the sequences before this round of kThreads
+  int base = 0;                                  // taken by the sequences before this round of kThreads
+  long long short_of = 0;                        // (what all ask for together may take more than 32 bits)
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + tid;
     Seq s{0, 0, 0, 0, 0, 0};
@@ -72,15 +74,15 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
       want = max(min(need, p.max_pages) - s.held, 0);
       lack = max(need - p.max_pages, 0);
     }
-    int before = want;
+    long long before = want;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, before, o);
+      const long long x = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += x;
     }
     if (lane == 31) s_warp[warp] = before;
     __syncthreads();
-    int all = 0;
+    long long all = 0;
     for (int w = 0; w < kWarps; ++w) {
       if (w == warp) before += all;
       all += s_warp[w];
@@ -88,9 +90,9 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
     const long long first = (long long)min(used, p.n_free) + base + before - want;
     s.first = (int)min(first, (long long)p.n_free);
     s.got = min(want, p.n_free - s.first);
-    short_of += want - s.got + lack;
+    short_of += (long long)want - s.got + lack;
     if (b < p.B) s_seq[b] = s;
-    base = min(base + all, p.n_free);            // nothing is left behind that point
+    base = (int)min(base + all, (long long)p.n_free);      // nothing is left behind that point
     __syncthreads();
   }
   for (int o = 16; o > 0; o >>= 1) short_of += __shfl_xor_sync(0xffffffffu, short_of, o);
@@ -199,9 +201,9 @@ __global__ void __launch_bounds__(kThreads) extend_tables_kernel(const __grid_co
   }
   if (cta == 0 && tid == 0) {
     p.free_used[0] = (int)min((long long)min(used, p.n_free) + base, (long long)p.n_free);
-    int n = 0;
+    long long n = 0;
     for (int w = 0; w < kWarps; ++w) n += s_want[w];
-    p.missing[0] = n;
+    p.missing[0] = (int)min(n, 0x7fffffffll);
   }
 }
 

@@ -21,7 +21,7 @@ class TablePlan(NamedTuple):
     seq_lens: torch.Tensor     #: int32 [B]: tokens of each sequence that this rank holds, the new ones among them
     draft_lens: torch.Tensor   #: int32 [B]: new ones of these (they are the last)
     mask: torch.Tensor         #: int64 [rows, mask_words]: bit i = the row's token descends from (or is) the i-th new local token
-    missing: torch.Tensor      #: int32 [1]: pages that the free list or the table had no room for
+    missing: torch.Tensor      #: int32 [1]: pages that the free list or the table had no room for (at most 2^31 - 1)
 
 
 def extend_tables(block_table: torch.Tensor, held: torch.Tensor, free_pages: torch.Tensor, free_used: torch.Tensor,

@@ -271,7 +271,7 @@ def extend_tables_reference(block_table, held, free_pages, free_used, ctx_lens, 
             for w in range(mask_words):
                 word = path >> (64 * w) & (2 ** 64 - 1)
                 mask[r0 + j, w] = word - 2 ** 64 if word >> 63 else word
-    return slots, positions, seq_lens, draft_lens, mask, torch.tensor([missing], dtype=torch.int32)
+    return slots, positions, seq_lens, draft_lens, mask, torch.tensor([min(missing, 2 ** 31 - 1)], dtype=torch.int32)
 
 
 def append_kv_reference(k, v, k_cache, v_cache, slots, hnd):
