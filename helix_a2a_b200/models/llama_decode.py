@@ -92,8 +92,6 @@ class HelixDecodeStack:
         self.held = torch.full((batch,), pages_per_seq, dtype=torch.int32, device=self.device)
         self.free_pages = perm[batch * pages_per_seq:].to(self.device)
         self.free_used = torch.zeros(1, dtype=torch.int32, device=self.device)
-        # pages and mask bits that were not to be had, over all calls so far (see check_room)
-        self.lost = torch.zeros(1, dtype=torch.int64, device=self.device)
         self.ctx_lens = torch.full((batch,), local_ctx * cp_size, dtype=torch.int32, device=self.device)
         shape = (self.n_pages, cfg.n_kv_heads, cfg.page_size, cfg.head_dim)
         self.k_cache: List[torch.Tensor] = []
@@ -170,52 +168,36 @@ class HelixDecodeStack:
 
     # ---- drafted tokens ---------------------------------------------------------------------------
     def _extend(self, q_start: torch.Tensor, rows: int, parents, mask_words: int) -> paged.TablePlan:
-        plan = paged.extend_tables(self.block_table, self.held, self.free_pages, self.free_used, self.ctx_lens, q_start, rows=rows,
+        return paged.extend_tables(self.block_table, self.held, self.free_pages, self.free_used, self.ctx_lens, q_start, rows=rows,
                                    page_size=self.cfg.page_size, parents=parents, mask_words=mask_words, cp_size=self.cp_size,
                                    cp_rank=self.cp_rank)
-        self.lost += plan.missing
-        if mask_words and rows > 64 * mask_words * self.cp_size:         # one sequence may have more tokens here than a mask has bits
-            self.lost += (plan.draft_lens - 64 * mask_words).clamp(min=0).sum()
-        return plan
-
-    def check_room(self) -> None:
-        """Raise if a :meth:`verify_step` or :meth:`commit` so far had tokens for which there was no page or no mask bit (waits for the
-        device).  From such a call on the outputs are wrong: tokens that are stored nowhere are counted, or do not see themselves."""
-        lost = int(self.lost)
-        if lost:
-            raise RuntimeError(f"this stack has outgrown draft_tokens={self.draft_tokens}: {lost} pages or mask bits were missing")
 
     def verify_step(self, q_all: torch.Tensor, k_all: torch.Tensor, v_all: torch.Tensor, q_start: torch.Tensor,
-                    parents: Optional[torch.Tensor] = None, *, max_new: int = 0) -> torch.Tensor:
+                    parents: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One pass over drafted tokens: ``q_all [L, rows, Hq, D]``, ``k_all`` / ``v_all [L, rows, Hkv, D]``, rows ``q_start[b]`` to
         ``q_start[b + 1]`` are sequence ``b``'s, ``parents [rows]`` their tree (``None``: chains), at most 256 of a sequence on a
-        rank; see :func:`ops.paged.extend_tables`.  ``max_new``: most tokens of one sequence in this step (0: unknown, up to
-        ``draft_tokens``); masks are made for so many, and the attention is divided by it.
+        rank; see :func:`ops.paged.extend_tables`.
         Returns ``y [L, rows, hidden]`` (this rank's partial sums).  Committed lengths stay as they are: the next call overwrites
         the drafted tokens, unless :meth:`commit` keeps some.  No host synchronisation, so the step can be captured.  ``plan`` holds
-        the step's places; :meth:`check_room` says whether all tokens of all steps had one."""
+        the step's places; where its ``missing`` is not 0 the stack has outgrown ``draft_tokens``, and its last tokens are nowhere."""
         if not self.draft_tokens:
             raise RuntimeError("this stack was made without draft_tokens")
-        if not 0 <= max_new <= min(self.draft_tokens, 256 * self.cp_size):
-            raise ValueError(f"max_new must be at most draft_tokens ({self.draft_tokens}) and 256 on a rank")
         rows = q_all.shape[1]
-        longest = max_new or max(min(self.draft_tokens, rows), 1)
-        words = min((longest + 64 * self.cp_size - 1) // (64 * self.cp_size), 4)       # a rank holds every cp_size-th token
+        words = min((self.draft_tokens + 63) // 64, 4)
         plan = self.plan = self._extend(q_start, rows, parents, words)
         ys = []
         for l in range(self.cfg.n_layers):
             paged.append_kv(k_all[l], v_all[l], self.k_cache[l], self.v_cache[l], plan.slots)
             with nvtx_range(f"layer{l}.tree_attention"):
                 o, lse = attention.tree_decode(q_all[l], self.k_cache[l], self.v_cache[l], self.block_table, plan.seq_lens, q_start,
-                                               plan.draft_lens, plan.mask, scale=self.scale, max_seq_len=self.max_local, max_q_len=longest)
+                                               plan.draft_lens, plan.mask, scale=self.scale, max_seq_len=self.max_local, max_q_len=self.draft_tokens)
             x = api.alltoall_combine(o, lse, self.workspace, self.cp_rank, self.cp_size) if self.cp_size > 1 else o
             ys.append(oproj_mod.oproj(x.reshape(rows, self.k_local), self._oproj_weight(l)))
         return torch.stack(ys)
 
     def commit(self, k_all: torch.Tensor, v_all: torch.Tensor, accepted: torch.Tensor, q_start: torch.Tensor) -> None:
         """Keep drafted tokens: ``accepted`` are their rows in ``k_all`` / ``v_all``, in the order of their positions, and ``q_start [B + 1]``
-        says which of them belong to which sequence.  A path through a tree becomes a run of tokens behind the committed ones.
-        Tokens without a page (:meth:`check_room`) count as committed all the same: lengths are those of all ranks."""
+        says which of them belong to which sequence.  A path through a tree becomes a run of tokens behind the committed ones."""
         if not self.draft_tokens:
             raise RuntimeError("this stack was made without draft_tokens")
         plan = self.plan = self._extend(q_start, accepted.numel(), None, 0)
