@@ -92,6 +92,8 @@ class HelixDecodeStack:
         self.held = torch.full((batch,), pages_per_seq, dtype=torch.int32, device=self.device)
         self.free_pages = perm[batch * pages_per_seq:].to(self.device)
         self.free_used = torch.zeros(1, dtype=torch.int32, device=self.device)
+        # pages and mask bits that were not to be had, over all calls so far (see check_room)
+        self.lost = torch.zeros(1, dtype=torch.int64, device=self.device)
         self.ctx_lens = torch.full((batch,), local_ctx * cp_size, dtype=torch.int32, device=self.device)
         shape = (self.n_pages, cfg.n_kv_heads, cfg.page_size, cfg.head_dim)
         self.k_cache: List[torch.Tensor] = []
@@ -168,9 +170,20 @@ class HelixDecodeStack:
 
     # ---- drafted tokens ---------------------------------------------------------------------------
     def _extend(self, q_start: torch.Tensor, rows: int, parents, mask_words: int) -> paged.TablePlan:
-        return paged.extend_tables(self.block_table, self.held, self.free_pages, self.free_used, self.ctx_lens, q_start, rows=rows,
+        plan = paged.extend_tables(self.block_table, self.held, self.free_pages, self.free_used, self.ctx_lens, q_start, rows=rows,
                                    page_size=self.cfg.page_size, parents=parents, mask_words=mask_words, cp_size=self.cp_size,
                                    cp_rank=self.cp_rank)
+        self.lost += plan.missing
+        if mask_words and rows > 64 * mask_words * self.cp_size:         # one sequence may have more tokens here than a mask has bits
+            self.lost += (plan.draft_lens - 64 * mask_words).clamp(min=0).sum()
+        return plan
+
+    def check_room(self) -> None:
+        """Raise if a :meth:`verify_step` or :meth:`commit` so far had tokens for which there was no page or no mask bit (waits for the
+        device).  From such a call on the outputs are wrong: tokens that are stored nowhere are counted, or do not see themselves."""
+        lost = int(self.lost)
+        if lost:
+            raise RuntimeError(f"this stack has outgrown draft_tokens={self.draft_tokens}: {lost} pages or mask bits were missing")
 
     def verify_step(self, q_all: torch.Tensor, k_all: torch.Tensor, v_all: torch.Tensor, q_start: torch.Tensor,
                     parents: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -179,7 +192,7 @@ class HelixDecodeStack:
         rank; see :func:`ops.paged.extend_tables`.
         Returns ``y [L, rows, hidden]`` (this rank's partial sums).  Committed lengths stay as they are: the next call overwrites
         the drafted tokens, unless :meth:`commit` keeps some.  No host synchronisation, so the step can be captured.  ``plan`` holds
-        the step's places; where its ``missing`` is not 0 the stack has outgrown ``draft_tokens``, and its last tokens are nowhere."""
+        the step's places; :meth:`check_room` says whether all tokens of all steps had one."""
         if not self.draft_tokens:
             raise RuntimeError("this stack was made without draft_tokens")
         rows = q_all.shape[1]
@@ -197,7 +210,8 @@ class HelixDecodeStack:
 
     def commit(self, k_all: torch.Tensor, v_all: torch.Tensor, accepted: torch.Tensor, q_start: torch.Tensor) -> None:
         """Keep drafted tokens: ``accepted`` are their rows in ``k_all`` / ``v_all``, in the order of their positions, and ``q_start [B + 1]``
-        says which of them belong to which sequence.  A path through a tree becomes a run of tokens behind the committed ones."""
+        says which of them belong to which sequence.  A path through a tree becomes a run of tokens behind the committed ones.
+        Tokens without a page (:meth:`check_room`) count as committed all the same: lengths are those of all ranks."""
         if not self.draft_tokens:
             raise RuntimeError("this stack was made without draft_tokens")
         plan = self.plan = self._extend(q_start, accepted.numel(), None, 0)
