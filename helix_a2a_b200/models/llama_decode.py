@@ -186,24 +186,28 @@ class HelixDecodeStack:
             raise RuntimeError(f"this stack has outgrown draft_tokens={self.draft_tokens}: {lost} pages or mask bits were missing")
 
     def verify_step(self, q_all: torch.Tensor, k_all: torch.Tensor, v_all: torch.Tensor, q_start: torch.Tensor,
-                    parents: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    parents: Optional[torch.Tensor] = None, *, max_new: int = 0) -> torch.Tensor:
         """One pass over drafted tokens: ``q_all [L, rows, Hq, D]``, ``k_all`` / ``v_all [L, rows, Hkv, D]``, rows ``q_start[b]`` to
         ``q_start[b + 1]`` are sequence ``b``'s, ``parents [rows]`` their tree (``None``: chains), at most 256 of a sequence on a
-        rank; see :func:`ops.paged.extend_tables`.
+        rank; see :func:`ops.paged.extend_tables`.  ``max_new``: most tokens of one sequence in this step (0: unknown, up to
+        ``draft_tokens``); masks are made for so many, and the attention is divided by it.
         Returns ``y [L, rows, hidden]`` (this rank's partial sums).  Committed lengths stay as they are: the next call overwrites
         the drafted tokens, unless :meth:`commit` keeps some.  No host synchronisation, so the step can be captured.  ``plan`` holds
         the step's places; :meth:`check_room` says whether all tokens of all steps had one."""
         if not self.draft_tokens:
             raise RuntimeError("this stack was made without draft_tokens")
+        if not 0 <= max_new <= min(self.draft_tokens, 256 * self.cp_size):
+            raise ValueError(f"max_new must be at most draft_tokens ({self.draft_tokens}) and 256 on a rank")
         rows = q_all.shape[1]
-        words = min((self.draft_tokens + 63) // 64, 4)
+        longest = max_new or max(min(self.draft_tokens, rows), 1)
+        words = min((longest + 64 * self.cp_size - 1) // (64 * self.cp_size), 4)       # a rank holds every cp_size-th token
         plan = self.plan = self._extend(q_start, rows, parents, words)
         ys = []
         for l in range(self.cfg.n_layers):
             paged.append_kv(k_all[l], v_all[l], self.k_cache[l], self.v_cache[l], plan.slots)
             with nvtx_range(f"layer{l}.tree_attention"):
                 o, lse = attention.tree_decode(q_all[l], self.k_cache[l], self.v_cache[l], self.block_table, plan.seq_lens, q_start,
-                                               plan.draft_lens, plan.mask, scale=self.scale, max_seq_len=self.max_local, max_q_len=self.draft_tokens)
+                                               plan.draft_lens, plan.mask, scale=self.scale, max_seq_len=self.max_local, max_q_len=longest)
             x = api.alltoall_combine(o, lse, self.workspace, self.cp_rank, self.cp_size) if self.cp_size > 1 else o
             ys.append(oproj_mod.oproj(x.reshape(rows, self.k_local), self._oproj_weight(l)))
         return torch.stack(ys)
