@@ -51,7 +51,9 @@ Tables extend_tables(torch::Tensor block_table, torch::Tensor held, torch::Tenso
   TORCH_CHECK(words >= 0 && words <= helix::kTableMaxWords, "mask_words must be 0 to ", helix::kTableMaxWords);
   TORCH_CHECK(page_size >= 1 && page_size <= (1 << 20), "page_size must be positive");
   TORCH_CHECK(cp_size >= 1 && cp_rank >= 0 && cp_rank < cp_size, "cp_rank must be in [0, cp_size)");
-  TORCH_CHECK(interleave >= 1 && interleave * cp_size <= (1 << 28), "interleave must be positive and interleave * cp_size at most 2^28");
+  constexpr int64_t kCycle = 1 << 28;
+  TORCH_CHECK(interleave >= 1 && interleave <= kCycle && cp_size <= kCycle && interleave * cp_size <= kCycle,
+              "interleave must be positive and interleave * cp_size at most 2^28");
   c10::cuda::CUDAGuard guard(dev);
   const auto i32 = [&](int64_t n) { return torch::Tensor(at::detail::empty_cuda({n}, at::kInt, dev, c10::nullopt)); };
   const auto i64 = [&](at::IntArrayRef n) { return torch::Tensor(at::detail::empty_cuda(n, at::kLong, dev, c10::nullopt)); };

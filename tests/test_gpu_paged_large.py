@@ -37,3 +37,11 @@ def test_more_pages_asked_for_than_32_bits_count():
     plan, table, held, used = plan_of((n, n, n), n, (5, 6, 7), 1, "cuda", rows_each=0)
     assert held.tolist() == [3, 0, 0] and int(used) == 3 and table[0, :4].tolist() == [5, 6, 7, 0] and not table[1:, :4].any()
     assert int(plan.missing) == END and plan.seq_lens.tolist() == [3, 0, 0]
+
+
+@pytest.mark.parametrize("cp_size,interleave", [(1, 2 ** 28 + 1), (4, 2 ** 62), (2 ** 62, 4), (2 ** 33, 2 ** 31), (2 ** 29, 1), (2, 2 ** 28)])
+def test_shares_that_leave_32_bits_are_refused(cp_size, interleave):
+    """... also where their product is a small number again in 64 bits."""
+    with pytest.raises(RuntimeError, match="2\\^28"):
+        paged.extend_tables(torch.zeros(1, 4, dtype=torch.int32, device="cuda"), ints(0), ints(1, 2, 3), ints(0), ints(5), ints(0, 2), rows=2,
+                            page_size=16, cp_size=cp_size, interleave=interleave)
