@@ -13,6 +13,9 @@
     python benchmarks/profile_case.py tree      # tree attention, B=8, 16 drafted tokens each, 16K tokens per sequence (537 MB of KV)
     python benchmarks/profile_case.py tree_wide # the same for one sequence of 64K tokens and 64 drafted ones (268 MB of KV)
     python benchmarks/profile_case.py int4      # o_proj with 4-bit weights, 100 tokens, K=8192, hidden 8192
+    python benchmarks/profile_case.py int4_few  # the same for 8 tokens
+    python benchmarks/profile_case.py append    # 16384 rows of K and V into a paged cache, a quarter of them other ranks' (101 MB moved)
+    python benchmarks/profile_case.py tables    # pages and slots of 64 prompts, 61000 tokens
 """
 import os
 import sys
@@ -48,6 +51,24 @@ def main():
         x = torch.randn(8, 8192, device="cuda").bfloat16()
         for _ in range(launches):
             oproj(x, w, splits=-1)
+    elif which == "append":
+        from helix_a2a_b200.ops import paged
+        qkv = torch.randn(16384, 3, 8, 128, device="cuda").half()
+        kc, vc = (torch.zeros(1024, 32, 8, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+        slots = torch.randperm(1024 * 32, device="cuda")[:16384]
+        slots[torch.rand(16384, device="cuda") < 0.25] = -1
+        for _ in range(launches):
+            paged.append_kv(qkv[:, 1], qkv[:, 2], kc, vc, slots, layout="NHD")
+    elif which == "tables":
+        from helix_a2a_b200.ops import paged
+        rows = 64 * 953
+
+        def zeros(*shape):
+            return torch.zeros(*shape, dtype=torch.int32, device="cuda")
+
+        free, starts = torch.randperm(64 * 64, device="cuda").int(), torch.arange(0, rows + 1, 953, device="cuda").int()
+        for _ in range(launches):
+            paged.extend_tables(zeros(64, 64), zeros(64), free, zeros(1), zeros(64), starts, rows=rows, page_size=16, mask_words=0)
     elif which in ("tree", "tree_wide"):
         from helix_a2a_b200.ops import attention, paged
         B, ctx, drafts = (8, 16384, 16) if which == "tree" else (1, 65536, 64)
@@ -64,10 +85,11 @@ def main():
         for _ in range(launches):
             attention.tree_decode(q, kc, vc, table, plan.seq_lens, i32(*range(0, B * drafts + 1, drafts)), plan.draft_lens, plan.mask,
                                   max_seq_len=ctx + drafts, max_q_len=drafts)
-    elif which == "int4":
+    elif which in ("int4", "int4_few"):
         from helix_a2a_b200.ops import oproj
-        w = oproj.quantize_weight_int4((torch.randn(8192, 8192, device="cuda") * 0.02).bfloat16())
-        x = torch.randn(100, 8192, device="cuda").bfloat16()
+        few = which == "int4_few"
+        w = oproj.quantize_weight_int4((torch.randn(8192, 8192, device="cuda") * 0.02).bfloat16(), zero_points=few)
+        x = torch.randn(8 if few else 100, 8192, device="cuda").bfloat16()
         for _ in range(launches):
             oproj.oproj(x, w)
     elif which == "combine":

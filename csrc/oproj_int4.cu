@@ -663,7 +663,7 @@ cudaError_t launch_oproj_int4(OprojInt4Params p, bool pdl, int sm_count, cudaStr
     return cudaErrorInvalidValue;
   int dev = 0;
   cudaGetDevice(&dev);
-  // Measured in graphs, 8192 x 8192: 8 tokens 12.1 us, 16 tokens 16.6 (two launches of eight 24), the other kernel 21.2 from 17 tokens on.  A
+  // Measured in graphs, 8192 x 8192: 8 tokens 11.9 us, 16 tokens 16.4 (two launches of eight 24), the other kernel 21.2 from 17 tokens on.  A
   // wider K than a cluster's warps hold takes the other kernel, too.
   if (p.tokens <= kInt4FewTokens && p.K <= kMaxCluster * kFewWarps * 256) return launch_few(p, pdl, sm_count, dev, stream);
   size_t smem = 0;

@@ -9,7 +9,8 @@
 // token L(p) and goes to slot table[L(p) / page] * page + L(p) % page.  Its mask holds a bit for each new local token on its
 // way to the root of the tree, itself included.
 //
-// The whole call is a few kilobytes, so what bounds it is the launch and a handful of dependent loads.  One cluster of up to
+// A step's call is a few kilobytes, so what bounds it is the launch and a handful of dependent loads (prompts: 61000 rows are 0.8 MB, and a
+// search and several divisions each, 10.0 us in a graph).  One cluster of up to
 // sixteen CTAs does it in one launch and without scratch memory: every CTA numbers all sequences for itself (three loads
 // per sequence), and a cluster barrier stands between everybody's reading of `held` and `free_used` and their update.
 #include "paged.h"
@@ -279,8 +280,8 @@ cudaError_t launch_extend_tables(const ExtendTablesParams& p, bool pdl, cudaStre
     if (e != cudaSuccess) return e;
     largest[dev] = there > 0 ? kMaxCtas : kPortable;
   }
-  // A row per thread, or a sequence per warp: one CTA for small calls, a cluster for large ones.  64 prompts, 61000 tokens, in a graph: 10.1 us
-  // with 16 CTAs, 17.2 with 8; 256 trees 6.7 and 9.5.
+  // A row per thread, or a sequence per warp: one CTA for small calls, a cluster for large ones.  64 prompts, 61000 tokens, in a graph: 10.0 us
+  // with 16 CTAs, 17.2 with 8; 256 trees 6.2 and 9.5.
   const int64_t work = p.parents ? ((int64_t)p.B + kWarps - 1) / kWarps : ((int64_t)p.rows + kThreads - 1) / kThreads;
   const int ctas = work > kPortable ? largest[dev].load() : (int)std::max<int64_t>(work, 1);
   cudaLaunchConfig_t cfg = config(dim3(ctas), dim3(kThreads), (size_t)std::max(p.B, 1) * sizeof(Seq), stream);

@@ -56,7 +56,9 @@ def tree_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     hold.  Returns what the exchange takes, ``o [rows, Hq, 128]`` and ``lse [rows, Hq]`` (fp32, natural log or base 2); a row that sees
     nothing, as rows behind ``q_start[B]`` do, is zero with LSE ``-inf``.
 
-    ``max_seq_len`` and ``max_q_len`` (0: unknown) only help to divide the work; results hold for any lengths.
+    ``max_seq_len`` and ``max_q_len`` (0: unknown), the longest sequence and the most rows of one, only help to divide the work; results hold for
+    any lengths.  Give ``max_q_len`` where a sequence has few of the call's rows: unknown, it is taken for all of them, and 64 sequences of five drafted tokens
+    then take 501 us instead of 371.
     """
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if layout not in ("HND", "NHD"):

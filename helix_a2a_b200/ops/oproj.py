@@ -30,7 +30,8 @@ def oproj(x: torch.Tensor, w, *, splits: int = 0, library: Optional[bool] = None
     kernel for every size.  Packed weights always use the hand-written kernel (the plain matrix is not kept).
 
     ``w`` may also be an :class:`Int4OprojWeight` (``splits`` and ``library`` have no meaning then): bf16 or fp16 ``x`` like its
-    scales, a quarter of the bytes.
+    scales, a quarter of the bytes.  That pays up to some 100 tokens: a launch has at most 128, each reads and unpacks all weights, and with 8192 x 8192
+    1024 tokens take 212 us where 16-bit weights take 90.  A group's products are added up in fp32 before its scale, so bf16 values beyond 10^35 overflow.
     """
     if isinstance(w, Int4OprojWeight):
         if not x.is_cuda:

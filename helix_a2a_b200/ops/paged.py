@@ -33,7 +33,7 @@ def extend_tables(block_table: torch.Tensor, held: torch.Tensor, free_pages: tor
     ``q_start [B + 1]``: rows ``q_start[b]`` to ``q_start[b + 1]`` are the new tokens of sequence ``b``, which follow its
     ``ctx_lens [B]`` committed ones (counted over all ranks).  ``q_start[0]`` is 0 and ``rows >= q_start[B]``; rows behind
     ``q_start[B]`` (a captured graph's padding) get slot -1, position 0 and an empty mask.  The token at place ``p`` of its sequence
-    belongs to rank ``p // interleave % cp_size``.  For a tree of drafted tokens ``parents [rows]`` holds the parent of each
+    belongs to rank ``p // interleave % cp_size`` (``interleave * cp_size`` at most 2^28).  For a tree of drafted tokens ``parents [rows]`` holds the parent of each
     (its number inside the sequence, smaller than the token's own; -1: the last committed token); without it every token follows the
     one before (a call with a tree has at most 2^20 rows).  The mask has ``64 * mask_words`` (at most 256) bits per row; new local tokens beyond that have none, and
     ``mask_words=0`` leaves the mask out (prompts).
